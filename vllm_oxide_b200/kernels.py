@@ -91,7 +91,7 @@ def _int32_vec(t: torch.Tensor, n: int, op: str, name: str) -> None:
 
 _fn_cache = {}
 _MODULES = ("elementwise", "gemm_f32", "gemm_sm100", "gemm_sm100_pair", "attention", "attention_mma", "attention_sm100", "sampling",
-            "streams", "recurrence", "latent_attention", "attention_flex", "moe")
+            "streams", "recurrence", "latent_attention", "attention_flex", "moe", "kv4")
 
 # Per-op device timing, off unless a profile is being taken: CUDA events around each wrapper
 # (the reference times ops by wall clock on the CPU and notes that a CUDA backend must use
@@ -2232,6 +2232,174 @@ DECODE_BALANCE_SEQS = 128        # most requests of a balanced decode launch
 def attn_decode_partial_floats(num_seqs: int, num_kv_heads: int, head_dim: int, splits: int) -> int:
     """Elements of the float32 scratch that `attn_decode_mma` needs for its merge through global memory."""
     return num_seqs * num_kv_heads * splits * (16 * head_dim + 32)
+
+
+# ------------------------------------------------------------------------------------ the cache in 4 bits
+def kv4_width(head_dim: int) -> int:
+    """Bytes that one token of one kv head takes in a 4-bit cache, key and value with their scales and minima. One layer's cache is
+    uint8 [pages, kv heads, page size, kv4_width(head_dim)]; what lies where inside a page: csrc/kv4.cuh."""
+    return 32 * -(-int(head_dim) // 32) + 8
+
+
+def kv4_supported(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether the kernels of the 4-bit cache take these sizes: heads a multiple of the kv heads, head sizes that are multiples of 16
+    up to 256, page sizes that are multiples of 8."""
+    return (num_kv_heads > 0 and num_heads > 0 and num_heads % num_kv_heads == 0 and 0 < head_dim <= 256 and head_dim % 16 == 0
+            and page_size > 0 and page_size % 8 == 0)
+
+
+def _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim):
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != num_kv_heads or cache.shape[3] != kv4_width(head_dim) \
+            or not cache.is_contiguous() or cache.shape[0] < 1:
+        raise ShapeError(op, f"the cache must be contiguous uint8 [pages, {num_kv_heads}, page_size, {kv4_width(head_dim)}], got "
+                             f"{cache.dtype} {list(cache.shape)}")
+    if cache.shape[0] * cache.shape[2] > 2 ** 31 - 1:
+        raise ShapeError(op, f"{cache.shape[0]} pages of {cache.shape[2]} tokens are beyond 2^31 - 1 slots")
+    if cache.data_ptr() % 16:
+        raise ShapeError(op, "the cache must start on a 16-byte boundary")
+    if not kv4_supported(num_heads, num_kv_heads, head_dim, cache.shape[2]):
+        raise ShapeError(op, f"sizes not supported: heads {num_heads}/{num_kv_heads}, head_dim {head_dim} (multiples of 16 up to 256), "
+                             f"page {cache.shape[2]} (multiples of 8)")
+
+
+def _kv4_rows(op, name, t, rows, cols, dtype):
+    _rows_2d(t, op, name)
+    if t.shape != (rows, cols) or t.dtype != dtype:
+        raise ShapeError(op, f"{name} must be {dtype} [{rows}, {cols}], got {t.dtype} {list(t.shape)}")
+
+
+@_timed
+def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: Optional[torch.Tensor],
+               inv_freq: Optional[torch.Tensor], cache: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+               q_out: Optional[torch.Tensor] = None) -> None:
+    """Rotate q (into `q_out`, or in place) and k (float32 angles position * inv_freq; None: no rotation) and put k, as rotated, and v
+    in 4 bits at their slots of `cache` (one layer's pages, see `kv4_width`). q [T, H*hd], k and v [T, KV*hd] may be column slices of one
+    wider tensor; k and v are left as they are. A token whose slot is negative (or `slots` None, or a slot behind the pool) is not
+    kept; no two tokens of one call may have the same slot. A key or value with a number that is not finite is kept as NaN."""
+    op = "kv4_append"
+    _cuda(op, q, k, v, positions, slots, inv_freq, cache, q_out)
+    _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
+    _rows_2d(q, op, "q")
+    T, code = q.shape[0], _code(q, op)
+    _kv4_rows(op, "q", q, T, num_heads * head_dim, q.dtype)
+    for name, t in (("k", k), ("v", v)):
+        _kv4_rows(op, name, t, T, num_kv_heads * head_dim, q.dtype)
+    if q_out is not None:
+        _kv4_rows(op, "q_out", q_out, T, num_heads * head_dim, q.dtype)
+    q_out = q if q_out is None else q_out
+    _int32_vec(positions, T, op, "positions")
+    if slots is not None:
+        _int32_vec(slots, T, op, "slots")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.shape != (head_dim // 2,) or not inv_freq.is_contiguous()):
+        raise ShapeError(op, f"inv_freq must be float32 [{head_dim // 2}], got {inv_freq.dtype} {list(inv_freq.shape)}")
+    f = _fn("kv4", "vob_kv4_append", [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P])
+    _check(f(_ptr(q), q.stride(0), _ptr(q_out), q_out.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(positions), _ptr(slots),
+             _ptr(inv_freq), _ptr(cache), cache.shape[0], code, T, num_heads, num_kv_heads, head_dim, cache.shape[2], _stream()),
+           op, 1 if T else 0)
+
+
+@_timed
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
+    """The keys (as rotated) and values that a 4-bit cache holds at `slots` (int32 [T]), as numbers: k_out, v_out [T, KV*hd], float32
+    or bfloat16. A negative slot gives zeros, one behind the pool NaN."""
+    op = "kv4_read"
+    _cuda(op, cache, slots, k_out, v_out)
+    _kv4_cache(op, cache, num_kv_heads, num_kv_heads, head_dim)
+    _rows_2d(k_out, op, "k_out")
+    T = k_out.shape[0]
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        _kv4_rows(op, name, t, T, num_kv_heads * head_dim, k_out.dtype)
+    _int32_vec(slots, T, op, "slots")
+    f = _fn("kv4", "vob_kv4_read", [_P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P])
+    _check(f(_ptr(cache), cache.shape[0], _ptr(slots), _ptr(k_out), k_out.stride(0), _ptr(v_out), v_out.stride(0), _code(k_out, op), T,
+             num_kv_heads, head_dim, cache.shape[2], _stream()), op, 1 if T else 0)
+
+
+class KV4Scratch:
+    """Scratch of `attn_decode_kv4`, where blocks that share a request's keys meet: made once (`kv4_scratch`), kept by whoever makes the
+    calls. The counters are zero between launches. Launches that use the same one must not run at the same time: one per stream,
+    and graphs that share one are replayed one behind the other."""
+
+    def __init__(self, partials: torch.Tensor, arrived: torch.Tensor):
+        self.partials, self.arrived = partials, arrived
+
+
+def _kv4_head_tiles(num_heads: int, num_kv_heads: int) -> int:
+    return -(-(num_heads // num_kv_heads) // 16)
+
+
+def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> KV4Scratch:
+    """What `attn_decode_kv4` needs for steps of at most `num_seqs` requests."""
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    units = max(1, num_seqs) * num_kv_heads * _kv4_head_tiles(num_heads, num_kv_heads)
+    return KV4Scratch(torch.empty(_kv4_partial_floats(head_dim, sms), dtype=torch.float32, device=device),
+                      torch.zeros(units, dtype=torch.int32, device=device))
+
+
+def _kv4_partial_floats(head_dim: int, sms: int) -> int:
+    return 2 * sms * 16 * (head_dim + 2)
+
+
+def _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window):
+    _cuda(op, q, out, cache, block_tables)
+    _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
+    _rows_2d(q, op, "q")
+    _code(q, op)
+    for name, t in (("q", q), ("out", out)):
+        _kv4_rows(op, name, t, q.shape[0], num_heads * head_dim, q.dtype)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+        raise ShapeError(op, "block_tables must be contiguous int32 [S, max_pages]")
+    if block_tables.shape[0] < num_seqs:
+        raise ShapeError(op, f"block_tables has {block_tables.shape[0]} rows for {num_seqs} requests")
+    if window < 0:
+        raise ShapeError(op, f"window {window} is negative")
+
+
+_KV4_ATTEND = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P]
+
+
+@_timed
+def attn_decode_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, positions: torch.Tensor,
+                    num_heads: int, num_kv_heads: int, head_dim: int, scale: float, window: int = 0, *, scratch: KV4Scratch) -> None:
+    """Attention of a step of single tokens over a 4-bit cache, row i belonging to request i at `positions[i]` (-1: a padding row,
+    which becomes 0). q, out [S, H*hd]; `window`: a row sees itself and the window - 1 tokens before it (0: every earlier token).
+    `scratch`: `kv4_scratch` for at least so many requests. A row whose page number lies outside the pool, or that sees a key or value
+    kept as NaN, becomes NaN."""
+    op = "attn_decode_kv4"
+    S = q.shape[0] if q.dim() == 2 else 0
+    _kv4_attn_checks(op, q, out, cache, block_tables, S, num_heads, num_kv_heads, head_dim, window)
+    _cuda(op, q, positions, scratch.partials, scratch.arrived)
+    _int32_vec(positions, S, op, "positions")
+    tiles = _kv4_head_tiles(num_heads, num_kv_heads)
+    sms = torch.cuda.get_device_properties(q.device).multi_processor_count
+    need = _kv4_partial_floats(head_dim, sms)
+    if scratch.partials.numel() < need or scratch.arrived.numel() < S * num_kv_heads * tiles:
+        raise ShapeError(op, f"the scratch is too small: made for {scratch.arrived.numel()} of {S * num_kv_heads * tiles} counters and "
+                             f"{scratch.partials.numel()} of {need} floats (see kv4_scratch)")
+    splits = max(1, min(32, 2 * sms // max(1, S * num_kv_heads * tiles)))
+    f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
+    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
+             _ptr(positions), _P(0), _P(0), S, 1, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), _code(q, op),
+             splits, _ptr(scratch.partials), _ptr(scratch.arrived), _stream()), op, 1 if S else 0)
+
+
+@_timed
+def attn_prefill_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_starts: torch.Tensor,
+                     context_lens: torch.Tensor, num_seqs: int, max_new: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                     scale: float, window: int = 0) -> None:
+    """Attention for portions of prompts and mixed batches over a 4-bit cache (which holds the step's own tokens too). q, out
+    [T, H*hd]; seq_starts int32 [S+1] (first row of each request), context_lens int32 [S] (tokens cached before the step), max_new = the
+    longest portion (a request's rows beyond it are not computed). `window` and what becomes NaN: as `attn_decode_kv4`. Rows that
+    belong to no request are left as they are."""
+    op = "attn_prefill_kv4"
+    _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window)
+    _cuda(op, q, seq_starts, context_lens)
+    _int32_vec(seq_starts, num_seqs + 1, op, "seq_starts")
+    _int32_vec(context_lens, num_seqs, op, "context_lens")
+    f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
+    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
+             _P(0), _ptr(seq_starts), _ptr(context_lens), num_seqs, max_new, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale),
+             int(window), _code(q, op), 1, _P(0), _P(0), _stream()), op, 1 if num_seqs > 0 and max_new > 0 else 0)
 
 
 # ------------------------------------------------------------------------------------ sampling
