@@ -88,12 +88,11 @@ ATTN = [dict(q=torch.zeros(3, 120)), dict(out=torch.zeros(3, 128, dtype=torch.bf
 
 
 @pytest.mark.parametrize("change", ATTN + [dict(positions=torch.zeros(2, dtype=torch.int32)),
-                                           dict(scratch=kernels.KV4Scratch(torch.zeros(10), torch.zeros(6, dtype=torch.int32))),
-                                           dict(scratch=kernels.KV4Scratch(torch.zeros(10 ** 6), torch.zeros(5, dtype=torch.int32)))])
+                                           dict(scratch=(2, 4, 2, 32)), dict(scratch=(3, 8, 2, 32)), dict(scratch=(3, 4, 2, 64))])
 def test_decode_refuses(no_gpu, change):
-    a = _attn_args(positions=torch.zeros(3, dtype=torch.int32),
-                   scratch=kernels.KV4Scratch(torch.zeros(10 ** 6), torch.zeros(6, dtype=torch.int32)))
+    a = _attn_args(positions=torch.zeros(3, dtype=torch.int32), scratch=(3, 4, 2, 32))
     a.update(change)
+    a["scratch"] = kernels.kv4_scratch(*a["scratch"], "cpu")
     with pytest.raises(ShapeError):
         kernels.attn_decode_kv4(**a)
 
@@ -104,3 +103,9 @@ def test_portions_refuse(no_gpu, change):
     a.update(change)
     with pytest.raises(ShapeError):
         kernels.attn_prefill_kv4(**a)
+
+
+def test_scratch_refuses(no_gpu):
+    for bad in ((-1, 4, 2, 32), (1, 3, 2, 32), (1, 4, 2, 24), (1, 4, 0, 32)):
+        with pytest.raises(ShapeError):
+            kernels.kv4_scratch(*bad, "cpu")

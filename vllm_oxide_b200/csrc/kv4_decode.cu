@@ -1,0 +1,668 @@
+// Attention of single tokens over the 4-bit cache (layout: kv4.cuh), bfloat16 activations, any head size up to 256.
+//
+// Math. With K_j = km_j + ks_j n_j and V_j = vm_j + vs_j w_j (codes n, w in 0 .. 15; one scale and minimum per vector):
+//   score_j = scale (ks_j (q . n_j) + km_j sum(q)),     p_j = 2^(score_j log2 e - M),
+//   out = (sum_j (p_j vs_j) w_j + sum_j p_j vm_j) / sum_j p_j.
+// Both products run on the codes themselves, by mma.sync in float16 with float32 sums; scales and minima come in once per
+// (head, key). A code needs no conversion: four bits alone in the low mantissa of a float16 are the number n 2^-24 (a subnormal, exact), four
+// bits one place higher 16 n 2^-24. So a 32-bit word of eight codes becomes four operand registers in five instructions (a shift by 8 and
+// four masks); the factors 16 are taken out of q (keys) and of the results (values).
+//   * q enters as float16: a bfloat16 has 8 bits and fits, times a power of two that brings the unit's largest number to 2^14 .. 2^15
+//     (numbers 2^28 below the largest start to lose bits).
+//   * p_j vs_j is rounded to float16, 11 bits (2^-12 of it on average less than bfloat16's 2^-9, which would be seen: the codes' sum is large
+//     against the result, which is the difference of it and the minima's). M is chosen from score_j log2 e + log2 vs_j, so that these products use
+//     float16's range from the top: at most 2^15, set to 2^4 when M moves. M moves only when a product would pass 2^15 (a vote per 32 keys;
+//     no reductions between lanes otherwise), and the sums so far are scaled once then.
+//   * sums of p_j, of p_j vm_j and of the products are float32.
+// Operands: S^T = N Q^T (A = 16 keys x 16 numbers straight from ldmatrix, B = Q^T, 8 heads) and O^T = W^T P^T (A = 16 numbers x 16 keys from
+// ldmatrix.trans, B = P^T by movmatrix of the scores' registers): eight heads a product fill an instruction that would be half empty with heads as rows.
+//
+// Work. The keys of all (request, kv head, heads) units, in rounds of 128, lie one behind the other; every block takes an equal share of
+// consecutive rounds, whatever the requests' lengths. In a round each of 4 warps has 32 keys, which it fetches itself (bulk copies of
+// 8 or 16 keys, contiguous whatever the page size, into a ring of its own: no barrier between warps until a unit ends). At the end of a unit's part
+// the warps' sums meet in shared memory; a unit that lies in several blocks is added up by the block that arrives last, in the order of the keys:
+// the result does not depend on which one that is.
+// Bound: memory (the codes are read once). 
+#include "kv4.cuh"
+VOB_PDL_SWITCH(kv4_decode)
+#include <cuda_fp16.h>
+#include "sm100.cuh"
+
+namespace {
+using namespace vob_kv4;
+using vob_sm100::smem_u32;
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int TILE = 32;                   // keys of a warp's step
+constexpr int ROUND = TILE * WARPS;        // keys of a block's step
+constexpr float P_LIMIT = 32768.f, P_TOP = 4.f;
+
+// NC chunks of 32 numbers, NT times 8 heads. Blocks per SM and stages of a warp's ring: as many bytes in flight as registers and
+// shared memory allow (4 blocks of 4 warps at head sizes up to 128).
+template <int NC, int NT> struct Sizes {
+    static constexpr int SUB = 256 * NC + 64;                     // bytes of eight keys and values
+    static constexpr int STAGE = SUB * (TILE / GROUP);
+    static constexpr int BLOCKS = NC > 4 || NC * NT > 4 ? 2 : NC * NT == 4 ? 3 : 4 - (NT - 1);
+    static constexpr int STAGES = NC <= 2 ? 5 : NC > 4 ? 3 : NT == 2 ? 5 : NC == 4 ? 4 : 3;
+    static constexpr int HEADS = 8 * NT;
+    static constexpr int OSTRIDE = 32 * NC + 8;                   // a head's sums in a stage, padded: 8 heads fill it exactly
+    static constexpr int PARTIAL = HEADS * (32 * NC + 2);         // floats of a partial result
+    static_assert(8 * OSTRIDE * 4 == STAGE, "the warps' sums of 8 heads use a stage of the ring");
+};
+
+struct Args {
+    const __nv_bfloat16* q;
+    long long q_stride;
+    __nv_bfloat16* out;
+    long long out_stride;
+    const unsigned char* cache;
+    const int* tables;
+    const int* positions;
+    float* partials;
+    int* arrived;
+    int* err;
+    int max_pages, num_pages, S, H, G, hd, page_size, window, head_tiles, table_keys;
+    float scale_log2;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A request's keys lo .. hi - 1, in rounds t0 .. t0 + count - 1. (A position behind the request's block table counts as one key behind it, which makes
+// the row NaN.)
+struct Span {
+    int lo, hi, t0, count;
+    __device__ __forceinline__ Span(int pos, int window, int table_keys) {
+        hi = min(max(pos, -1), table_keys) + 1;
+        lo = window ? max(0, hi - window) : 0;
+        t0 = lo / ROUND;
+        count = hi > 0 ? (hi + ROUND - 1) / ROUND - t0 : 0;
+    }
+};
+
+// A place in the order of rounds: round k of unit `gh` (kv head, heads) of request s.
+struct Place {
+    int s, gh, k;
+};
+
+template <int NC, int NT>
+__global__ void __launch_bounds__(THREADS, Sizes<NC, NT>::BLOCKS)
+kv4_decode_kernel(const Args a) {
+    using Z = Sizes<NC, NT>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char* ring = smem;                                                    // [WARPS][STAGES][STAGE]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * Z::STAGES * Z::STAGE);    // [WARPS][STAGES]
+    float* sM = reinterpret_cast<float*>(bars + WARPS * Z::STAGES);                // [WARPS][HEADS] reference, then sums of p, of p vm
+    float* sL = sM + WARPS * Z::HEADS;
+    float* sB = sL + WARPS * Z::HEADS;
+    int* sFlag = reinterpret_cast<int*>(sB + WARPS * Z::HEADS);
+    int* s_last = sFlag + 1;
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
+    const int GH = a.G * a.head_tiles, group = a.H / a.G;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < WARPS * Z::STAGES; ++i) vob_sm100::mbar_init(bars + i, 1);
+        *sFlag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // The order of the work: rounds of all requests, and where this block's share begins (every warp for itself; the positions were there
+    // before the step's first kernel).
+    Place at = {0, 0, 0};
+    int x0, x1, share;
+    {
+        const int per = (a.S + 31) / 32, s_lo = min(a.S, lane * per), s_hi = min(a.S, s_lo + per);
+        int mine = 0;
+        for (int s = s_lo; s < s_hi; ++s) mine += Span(a.positions[s], a.window, a.table_keys).count;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const int total = __shfl_sync(0xffffffffu, incl, 31) * GH;
+        share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+        x0 = (int)min((long long)total, (long long)share * blockIdx.x);
+        x1 = min(total - x0, share) + x0;
+        const int before = (incl - mine) * GH;
+        const bool here = before <= x0 && x0 < incl * GH;
+        if (here) {
+            int left = x0 - before;
+            for (int s = s_lo;; ++s) {
+                const int count = Span(a.positions[s], a.window, a.table_keys).count;
+                if (left < count * GH) {
+                    at = {s, left / count, left % count};
+                    break;
+                }
+                left -= count * GH;
+            }
+        }
+        const int src = max(0, __ffs(__ballot_sync(0xffffffffu, here)) - 1);
+        at.s = __shfl_sync(0xffffffffu, at.s, src);
+        at.gh = __shfl_sync(0xffffffffu, at.gh, src);
+        at.k = __shfl_sync(0xffffffffu, at.k, src);
+    }
+    __syncthreads();
+    pdl_wait(33);
+    // padding rows see nothing
+    for (int s = blockIdx.x * WARPS + warp; s < a.S; s += gridDim.x * WARPS)
+        if (a.positions[s] < 0)
+            for (int i = lane; i < a.H * a.hd; i += 32) a.out[(size_t)s * a.out_stride + i] = __float2bfloat16_rn(0.f);
+    if (x0 >= x1) return;
+
+    const int piece = a.page_size % 16 ? 8 : 16, pieces = TILE / piece;            // keys of one copy: eight lie together, more inside a page
+    const uint32_t piece_bytes = (uint32_t)(piece / 8) * Z::SUB;
+    const int width = 32 * NC + 8;
+    unsigned char* my_ring = ring + warp * Z::STAGES * Z::STAGE;
+    const uint32_t ring_at = smem_u32(my_ring), bar_at = smem_u32(bars + warp * Z::STAGES);
+
+    // ---------------------------------------------------------------- fetching
+    Place ld = at;                                                                 // the next round to fetch from
+    int ld_x = x0;
+    Span ld_span(a.positions[ld.s], a.window, a.table_keys);
+    int batch_k = -1, batch_end = -1;                                              // rounds of the unit whose pages the lanes hold
+    int page = 0, page_off = 0;                                                    // of piece lane % pieces of round batch_k + lane / pieces
+    int stage_in = 0, issued = 0, taken = 0;
+    bool dead = false;                                                              // a wait ran out: nothing more is fetched or waited for
+    auto fetch = [&]() {
+        while (ld_x < x1 && !dead) {
+            const int base = (ld_span.t0 + ld.k) * ROUND + warp * TILE;
+            const bool any = base < ld_span.hi && base + TILE > ld_span.lo;
+            if (any) {
+                const int per_batch = 32 / pieces;
+                if (batch_k < 0 || ld.k >= batch_end) {
+                    batch_k = ld.k;
+                    batch_end = batch_k + per_batch;
+                    const int key = (ld_span.t0 + batch_k + lane / pieces) * ROUND + warp * TILE + (lane % pieces) * piece;
+                    const int idx = key / a.page_size;
+                    page_off = key - idx * a.page_size;
+                    page = -2;                                                      // nothing to fetch
+                    if (key < ld_span.hi && key + piece > ld_span.lo) page = idx < a.max_pages ? a.tables[(size_t)ld.s * a.max_pages + idx] : -1;
+                }
+                const bool mine = lane / pieces == ld.k - batch_k;
+                const bool want = mine && page != -2, good = want && page >= 0 && page < a.num_pages;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * piece_bytes;
+                const uint32_t bar = bar_at + 8 * stage_in, dst = ring_at + stage_in * Z::STAGE + (lane % pieces) * piece_bytes;
+                if (__any_sync(0xffffffffu, want && !good)) {
+                    // a page outside the pool: NaN where its scales would be
+                    if (want && !good)
+                        for (int i = 0; i < piece; ++i)
+                            *reinterpret_cast<uint2*>(my_ring + stage_in * Z::STAGE + (lane % pieces) * piece_bytes + (i >> 3) * Z::SUB + 256 * NC + 8 * (i & 7)) =
+                                make_uint2(0x7fff7fffu, 0x7fff7fffu);
+                    vob_sm100::fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) vob_sm100::mbar_expect_tx(bars + warp * Z::STAGES + stage_in, bytes);
+                __syncwarp();
+                if (good)
+                    bulk_load(dst, a.cache + (((size_t)page * a.G + ld.gh / a.head_tiles) * a.page_size + page_off) * width, piece_bytes, bar);
+                stage_in = stage_in + 1 == Z::STAGES ? 0 : stage_in + 1;
+                ++issued;
+            }
+            ++ld_x;
+            if (++ld.k == ld_span.count) {
+                ld.k = 0;
+                batch_k = -1;
+                if (++ld.gh == GH) {
+                    ld.gh = 0;
+                    while (ld_x < x1) {
+                        ld_span = Span(a.positions[++ld.s], a.window, a.table_keys);
+                        if (ld_span.count) break;
+                    }
+                }
+            }
+            if (any) return;
+        }
+    };
+#pragma unroll 1
+    for (int i = 0; i < Z::STAGES - 1; ++i) fetch();
+
+    // ---------------------------------------------------------------- units
+    int stage_out = 0;
+    uint32_t phase = 0;
+    int x = x0;
+    while (x < x1) {
+        const Span span(a.positions[at.s], a.window, a.table_keys);
+        const int kvh = at.gh / a.head_tiles, head0 = kvh * group + (at.gh % a.head_tiles) * Z::HEADS;
+        const int heads = min(Z::HEADS, kvh * group + group - head0);
+        const int k_end = min(span.count, at.k + (x1 - x));
+        // Q^T as the B operand: lane (head g8, c4) holds numbers 32c + 8 c4 + {0,4}, {1,5} / 16, {2,6}, {3,7} / 16 of each chunk
+        uint32_t qf[NT][NC][4];
+        float qs[NT][2];
+        float to_score;                                                             // scale log2 e 2^24 / (the power of two that q was given)
+        {
+            float sum[NT], big = 0.f;
+            uint4 raw[NT][NC];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int h = 8 * n + g8;
+                sum[n] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int d = 32 * c + 8 * c4;
+                    raw[n][c] = make_uint4(0, 0, 0, 0);
+                    if (h < heads && d < a.hd)
+                        raw[n][c] = *reinterpret_cast<const uint4*>(a.q + (size_t)at.s * a.q_stride + (size_t)(head0 + h) * a.hd + d);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const uint32_t w[4] = {raw[n][c].x, raw[n][c].y, raw[n][c].z, raw[n][c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xffff0000u);
+                        sum[n] += lo + hi;
+                        big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+                    }
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            int e = 0;                                                               // 2^(14 - e) <= 1 / big < 2^(15 - e)
+            if (big > 0.f && big < INFINITY) e = max(-100, min(100, ilogbf(big)));
+            const float up = exp2f((float)(14 - e));
+            to_score = a.scale_log2 * exp2f((float)(10 + e));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const uint32_t w[4] = {raw[n][c].x, raw[n][c].y, raw[n][c].z, raw[n][c].w};
+                    float f[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16) * up; f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * up; }
+                    qf[n][c][0] = pack_half2(f[0], f[4]);
+                    qf[n][c][1] = pack_half2(f[1] * 0.0625f, f[5] * 0.0625f);
+                    qf[n][c][2] = pack_half2(f[2], f[6]);
+                    qf[n][c][3] = pack_half2(f[3] * 0.0625f, f[7] * 0.0625f);
+                }
+                float t = sum[n] * a.scale_log2;
+                t += __shfl_xor_sync(0xffffffffu, t, 1);
+                t += __shfl_xor_sync(0xffffffffu, t, 2);
+                qs[n][0] = __shfl_sync(0xffffffffu, t, 8 * c4);                      // heads 2 c4 and 2 c4 + 1: the scores' columns
+                qs[n][1] = __shfl_sync(0xffffffffu, t, 8 * c4 + 4);
+            }
+        }
+        float ref[NT][2], l[NT][2], base_v[NT][2], o[NT][NC][2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { ref[n][i] = -INFINITY; l[n][i] = 0.f; base_v[n][i] = 0.f; }
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][c][0][i] = o[n][c][1][i] = 0.f;
+        }
+        bool worked = false;
+        int my_stage = 0;
+        for (int k = at.k; k < k_end; ++k) {
+            const int base = (span.t0 + k) * ROUND + warp * TILE;
+            if (!(base < span.hi && base + TILE > span.lo)) continue;
+            fetch();                                                                 // into the stage of the tile before this one
+            if (!dead && __any_sync(0xffffffffu, !vob_sm100::mbar_wait(bars + warp * Z::STAGES + stage_out, phase, sFlag, a.err, 31))) {
+                dead = true;
+                // what is in flight lands before the block ends
+                for (int i = taken; i < issued; ++i) {
+                    const unsigned long long t0 = vob_sm100::global_ns();
+                    while (!vob_sm100::mbar_try_wait(bars + warp * Z::STAGES + i % Z::STAGES, (i / Z::STAGES) & 1) &&
+                           vob_sm100::global_ns() - t0 < vob_sm100::WAIT_LIMIT_NS) {}
+                }
+            }
+            ++taken;
+            my_stage = stage_out;
+            const unsigned char* st = my_ring + stage_out * Z::STAGE;
+            const uint32_t st_at = ring_at + stage_out * Z::STAGE;
+            if (++stage_out == Z::STAGES) { stage_out = 0; phase ^= 1; }
+            worked = true;
+
+            // scores of 32 keys: two tiles of 16
+            float s[2][NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[0][n][i] = s[1][n][i] = 0.f;
+            const uint32_t row_at = st_at + (lane >> 3) * Z::SUB + (lane & 7) * 16;   // matrix lane / 8 = eight keys
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                uint32_t w[4];
+                ldsm4(w, row_at + 128 * c);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        mma(s[t][n], w[2 * t] & 0x000f000fu, w[2 * t + 1] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x00f000f0u,
+                            qf[n][c][0], qf[n][c][1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] >>= 8;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        mma(s[t][n], w[2 * t] & 0x000f000fu, w[2 * t + 1] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x00f000f0u,
+                            qf[n][c][2], qf[n][c][3]);
+            }
+            // scales and minima of this lane's keys g8, g8 + 8, + 16, + 24
+            float2 ks[4], vs[4];
+            float vt[4];                                                             // the value's scale, as the reference takes it
+            bool seen[4] = {true, true, true, true};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint2 w = *reinterpret_cast<const uint2*>(st + i * Z::SUB + 256 * NC + 8 * g8);
+                ks[i] = scale_min(w.x);
+                vs[i] = scale_min(w.y);
+                ks[i].x *= to_score;
+            }
+            const bool edge = base < span.lo || base + TILE > span.hi;
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = base + 8 * i + g8;
+                    seen[i] = j >= span.lo && j < span.hi;
+                    if (!seen[i]) { ks[i] = make_float2(0.f, 0.f); vs[i] = make_float2(0.f, 0.f); }   // whatever lies there
+                }
+            }
+            // below 2^-40 a scale counts as that: p itself stays below 2^55, whatever the values of the keys with large scores
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vt[i] = vs[i].x < 9.094947e-13f ? 9.094947e-13f : vs[i].x;
+            float p[2][NT][4];
+            bool over = false;
+            auto weigh = [&](int n) {
+                bool past = false;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 2 * t + (i >> 1);
+                        float e = exp2_fast(fmaf(s[t][n][i], ks[key].x, fmaf(ks[key].y, qs[n][i & 1], -ref[n][i & 1])));
+                        if (edge && !seen[key]) e = 0.f;
+                        p[t][n][i] = e;
+                        past = past || !(e * vt[key] <= P_LIMIT);
+                    }
+                return past;
+            };
+#pragma unroll
+            for (int n = 0; n < NT; ++n) over = weigh(n) || over;
+            if (__any_sync(0xffffffffu, over)) {
+                // a new reference: the largest score + log2 of its value's scale
+                float lg[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lg[i] = log2f(vt[i]) - P_TOP;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = 2 * t + (i >> 1);
+                            const float y = fmaf(s[t][n][i], ks[key].x, ks[key].y * qs[n][i & 1]) + lg[key];
+                            if (seen[key]) top[i & 1] = fmaxf(top[i & 1], y);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+                        const float to = fmaxf(ref[n][i], top[i]);
+                        const float f = ref[n][i] == -INFINITY ? 0.f : exp2_fast(ref[n][i] - to);
+                        ref[n][i] = to;
+                        l[n][i] *= f;
+                        base_v[n][i] *= f;
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) { o[n][c][m][i] *= f; o[n][c][m][2 + i] *= f; }
+                    }
+                    weigh(n);
+                }
+            }
+            uint32_t pb[NT][2][2];                                                   // P^T as the B operand
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 2 * t + (i >> 1);
+                        l[n][i & 1] += p[t][n][i];
+                        base_v[n][i & 1] = fmaf(p[t][n][i], vs[key].y, base_v[n][i & 1]);
+                    }
+                    pb[n][t][0] = transpose8(pack_half2(p[t][n][0] * vs[2 * t].x, p[t][n][1] * vs[2 * t].x));
+                    pb[n][t][1] = transpose8(pack_half2(p[t][n][2] * vs[2 * t + 1].x, p[t][n][3] * vs[2 * t + 1].x));
+                }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                uint32_t w[4];
+                ldsm4_trans(w, row_at + 128 * (NC + c));
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            mma(o[n][c][m], w[2 * t] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x000f000fu, w[2 * t + 1] & 0x00f000f0u,
+                                pb[n][t][0], pb[n][t][1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] >>= 8;
+                }
+            }
+            __syncwarp();                                                            // every lane has read the stage: it may be fetched into
+        }
+
+        // ------------------------------------------------------------ the unit's part ends: the warps' sums meet
+        const bool whole = at.k == 0 && k_end == span.count;
+        float* part = a.partials + (size_t)(2 * blockIdx.x + (x == x0 ? 0 : 1)) * Z::PARTIAL;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], off);
+                    base_v[n][i] += __shfl_xor_sync(0xffffffffu, base_v[n][i], off);
+                }
+                if (g8 == 0) {
+                    const int h = warp * Z::HEADS + 8 * n + 2 * c4 + i;
+                    sM[h] = ref[n][i];
+                    sL[h] = worked ? l[n][i] : 0.f;
+                    sB[h] = base_v[n][i];
+                }
+            }
+        }
+        int* s_stage = s_last + 1;                                                   // [WARPS] the stage a warp's sums lie in, -1: it had no keys
+        if (lane == 0) s_stage[warp] = worked ? my_stage : -1;
+        for (int n = 0; n < NT; ++n) {
+            if (worked) {
+                // sums of 8 heads over the tile just read (its stage is fetched into only after the next tile's wait)
+                float* dst = reinterpret_cast<float*>(my_ring + my_stage * Z::STAGE);
+#pragma unroll
+                for (int nn = 0; nn < NT; ++nn)
+                    if (nn == n) {
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                *reinterpret_cast<float4*>(dst + (2 * c4 + i) * Z::OSTRIDE + 32 * c + 4 * g8) =
+                                    make_float4(o[nn][c][0][i], o[nn][c][0][2 + i], o[nn][c][1][i], o[nn][c][1][2 + i]);
+                    }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 8 * 8 * NC; i += THREADS) {
+                const int h8 = i / (8 * NC), d = 4 * (i % (8 * NC)), h = 8 * n + h8;
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sM[w * Z::HEADS + h]);
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f, mins = 0.f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    if (s_stage[w] < 0) continue;
+                    const float mw = sM[w * Z::HEADS + h];
+                    // (a warp whose keys all gave NaN has no reference: its sums are NaN and stay so)
+                    const float f = mw == -INFINITY ? 1.f : exp2_fast(mw - m);
+                    const float4 v = *reinterpret_cast<const float4*>(ring + (w * Z::STAGES + s_stage[w]) * Z::STAGE + (h8 * Z::OSTRIDE + d) * 4);
+                    acc.x = fmaf(f, v.x, acc.x);
+                    acc.y = fmaf(f, v.y, acc.y);
+                    acc.z = fmaf(f, v.z, acc.z);
+                    acc.w = fmaf(f, v.w, acc.w);
+                    sum = fmaf(f, sL[w * Z::HEADS + h], sum);
+                    mins = fmaf(f, sB[w * Z::HEADS + h], mins);
+                }
+                // codes entered as n 2^-24, those in the high four bits of a byte as 16 n 2^-24
+                acc.x = fmaf(acc.x, 16777216.f, mins);
+                acc.y = fmaf(acc.y, 1048576.f, mins);
+                acc.z = fmaf(acc.z, 16777216.f, mins);
+                acc.w = fmaf(acc.w, 1048576.f, mins);
+                if (whole) {
+                    if (h < heads && d < a.hd) {
+                        const float inv = 1.f / sum;
+                        __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)at.s * a.out_stride + (size_t)(head0 + h) * a.hd + d);
+                        dst[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+                        dst[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                    }
+                } else {
+                    *reinterpret_cast<float4*>(part + h * (32 * NC) + d) = acc;
+                    if (d == 0) {
+                        part[Z::HEADS * 32 * NC + h] = m;
+                        part[Z::HEADS * 32 * NC + Z::HEADS + h] = sum;
+                    }
+                }
+            }
+            vob_sm100::fence_proxy_async_smem();                                      // the stages go back to the copies
+            __syncthreads();
+        }
+        if (!whole) {
+            // the unit's rounds begin at x - at.k; blocks c0 .. c1 have parts of it
+            const int b0 = x - at.k;
+            const int c0 = b0 / share, c1 = (b0 + span.count - 1) / share;
+            const int unit = at.s * GH + at.gh;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const bool is_last = atomicAdd(a.arrived + unit, 1) == c1 - c0;
+                if (is_last) a.arrived[unit] = 0;                                     // as it was found, for the next launch
+                *s_last = is_last;
+            }
+            __syncthreads();
+            if (*s_last) {
+                __threadfence();
+                for (int i = threadIdx.x; i < Z::HEADS * 8 * NC; i += THREADS) {
+                    const int h = i / (8 * NC), d = 4 * (i % (8 * NC));
+                    if (h >= heads || d >= a.hd) continue;
+                    float m = -INFINITY, sum = 0.f;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int c = c0; c <= c1; ++c) {
+                        const float* from = a.partials + (size_t)(2 * c + (share * c >= b0 ? 0 : 1)) * Z::PARTIAL;
+                        m = fmaxf(m, __ldcg(from + Z::HEADS * 32 * NC + h));
+                    }
+                    for (int c = c0; c <= c1; ++c) {
+                        const float* from = a.partials + (size_t)(2 * c + (share * c >= b0 ? 0 : 1)) * Z::PARTIAL;
+                        const float mc = __ldcg(from + Z::HEADS * 32 * NC + h);
+                        const float f = mc == -INFINITY ? 1.f : exp2_fast(mc - m);
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + h * (32 * NC) + d));
+                        acc.x = fmaf(f, v.x, acc.x);
+                        acc.y = fmaf(f, v.y, acc.y);
+                        acc.z = fmaf(f, v.z, acc.z);
+                        acc.w = fmaf(f, v.w, acc.w);
+                        sum = fmaf(f, __ldcg(from + Z::HEADS * 32 * NC + Z::HEADS + h), sum);
+                    }
+                    const float inv = 1.f / sum;
+                    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)at.s * a.out_stride + (size_t)(head0 + h) * a.hd + d);
+                    dst[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+                    dst[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                }
+            }
+        }
+        x += k_end - at.k;
+        at.k = 0;
+        if (x < x1 && ++at.gh == GH) {
+            at.gh = 0;
+            do ++at.s; while (Span(a.positions[at.s], a.window, a.table_keys).count == 0);
+        }
+    }
+}
+
+template <int NC, int NT> constexpr size_t smem_bytes() {
+    using Z = Sizes<NC, NT>;
+    return (size_t)WARPS * Z::STAGES * Z::STAGE + WARPS * Z::STAGES * 8 + 3 * WARPS * Z::HEADS * 4 + 4 * (2 + WARPS);
+}
+
+template <int NC, int NT> int launch(const Args& a, long long max_rounds, int sms, long long partial_floats, cudaStream_t stream) {
+    using Z = Sizes<NC, NT>;
+    if (partial_floats < 2LL * sms * Z::BLOCKS * Z::PARTIAL) return VOB_ERR_BAD_ARG;
+    static char done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(kv4_decode_kernel<NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NC, NT>());
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) done[dev] = 1;
+    }
+    const long long most = (long long)a.S * a.G * a.head_tiles * max_rounds;
+    const int grid = (int)min(most, (long long)sms * Z::BLOCKS);
+    return vob_launch(kv4_decode_kernel<NC, NT>, dim3(max(grid, 1)), dim3(THREADS), smem_bytes<NC, NT>(), stream, a);
+}
+
+int heads_per_unit(int group, int hd) { return group > 8 && hd <= 128 ? 16 : 8; }
+
+}  // namespace
+
+// q [S, H * hd] bfloat16, rows 16-byte aligned; out likewise, rows 4-byte aligned; positions int32 [S]. `partials`: two parts per block that the SMs
+// hold (`partial_floats` of them are there); `arrived`: a zero per request, kv head and 8 (16) heads.
+VOB_EXPORT int vob_kv4_decode(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, long long num_pages,
+                              const int* tables, int max_pages, const int* positions, int S, int H, int G, int hd, int page_size, float scale,
+                              int window, float* partials, long long partial_floats, int* arrived, long long counters, int sms, int* err, cudaStream_t stream) {
+    if (S <= 0) return 0;
+    if (H <= 0 || G <= 0 || H % G || hd <= 0 || hd % 16 || hd > 256 || page_size <= 0 || page_size % 8 || num_pages <= 0 || num_pages > 0x7fffffffLL ||
+        max_pages <= 0 || window < 0 || sms <= 0 || !partials || !arrived)
+        return VOB_ERR_BAD_ARG;
+    if (((uintptr_t)q & 15) || q_stride % 8 || ((uintptr_t)out & 3) || out_stride % 2 || ((uintptr_t)cache & 15) || ((uintptr_t)partials & 15)) return VOB_ERR_BAD_ARG;
+    Args a = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache, tables, positions, partials, arrived, err,
+              max_pages, (int)num_pages, S, H, G, hd, page_size, window, 0, 0, scale * 1.4426950408889634f};
+    const int heads = heads_per_unit(H / G, hd);
+    a.head_tiles = (H / G + heads - 1) / heads;
+    if (counters < (long long)S * G * a.head_tiles) return VOB_ERR_BAD_ARG;
+    const long long keys = window ? min((long long)max_pages * page_size, (long long)window) : (long long)max_pages * page_size;
+    const long long rounds = keys / ROUND + 2;
+    if ((long long)max_pages * page_size > 0x7ffffff0LL || rounds * S * G * a.head_tiles > 0x7fffffffLL) return VOB_ERR_UNSUPPORTED;
+    a.table_keys = max_pages * page_size;
+    switch (chunks(hd) * 2 + (heads == 16)) {
+        case 2: return launch<1, 1>(a, rounds, sms, partial_floats, stream);
+        case 3: return launch<1, 2>(a, rounds, sms, partial_floats, stream);
+        case 4: return launch<2, 1>(a, rounds, sms, partial_floats, stream);
+        case 5: return launch<2, 2>(a, rounds, sms, partial_floats, stream);
+        case 6: return launch<3, 1>(a, rounds, sms, partial_floats, stream);
+        case 7: return launch<3, 2>(a, rounds, sms, partial_floats, stream);
+        case 8: return launch<4, 1>(a, rounds, sms, partial_floats, stream);
+        case 9: return launch<4, 2>(a, rounds, sms, partial_floats, stream);
+        case 10: return launch<5, 1>(a, rounds, sms, partial_floats, stream);
+        case 12: return launch<6, 1>(a, rounds, sms, partial_floats, stream);
+        case 14: return launch<7, 1>(a, rounds, sms, partial_floats, stream);
+        case 16: return launch<8, 1>(a, rounds, sms, partial_floats, stream);
+    }
+    return VOB_ERR_UNSUPPORTED;
+}

@@ -91,7 +91,7 @@ def _int32_vec(t: torch.Tensor, n: int, op: str, name: str) -> None:
 
 _fn_cache = {}
 _MODULES = ("elementwise", "gemm_f32", "gemm_sm100", "gemm_sm100_pair", "attention", "attention_mma", "attention_sm100", "sampling",
-            "streams", "recurrence", "latent_attention", "attention_flex", "moe", "kv4")
+            "streams", "recurrence", "latent_attention", "attention_flex", "moe", "kv4", "kv4_decode")
 
 # Per-op device timing, off unless a profile is being taken: CUDA events around each wrapper
 # (the reference times ops by wall clock on the CPU and notes that a CUDA backend must use
@@ -924,7 +924,7 @@ def gemm_sm100_check() -> None:
             sc.err.zero_()
             raise KernelError(f"a bounded wait expired inside a tensor-core kernel (code {code}: 1-4 = matrix product: TMA "
                               "producer, MMA issuer, epilogue, peers of a split; 11-21 = attention: 11-12 TMA producer, 13-17 MMA issuer, "
-                              "18-21 softmax rows); its result is not valid")
+                              "18-21 softmax rows; 31 = decode attention over a 4-bit cache); its result is not valid")
 
 
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None, fixed_w: bool = False) -> None:
@@ -2320,24 +2320,20 @@ class KV4Scratch:
     calls. The counters are zero between launches. Launches that use the same one must not run at the same time: one per stream,
     and graphs that share one are replayed one behind the other."""
 
-    def __init__(self, partials: torch.Tensor, arrived: torch.Tensor):
-        self.partials, self.arrived = partials, arrived
-
-
-def _kv4_head_tiles(num_heads: int, num_kv_heads: int) -> int:
-    return -(-(num_heads // num_kv_heads) // 16)
+    def __init__(self, num_seqs: int, sizes: tuple, sms: int, partials: torch.Tensor, arrived: torch.Tensor):
+        self.num_seqs, self.sizes, self.sms, self.partials, self.arrived = num_seqs, sizes, sms, partials, arrived
 
 
 def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> KV4Scratch:
-    """What `attn_decode_kv4` needs for steps of at most `num_seqs` requests."""
+    """What `attn_decode_kv4` needs for steps of at most `num_seqs` requests of these sizes."""
+    if not kv4_supported(num_heads, num_kv_heads, head_dim, 8) or num_seqs < 0:
+        raise ShapeError("kv4_scratch", f"sizes not supported: {num_seqs} requests, heads {num_heads}/{num_kv_heads}, head_dim {head_dim}")
     sms = torch.cuda.get_device_properties(device).multi_processor_count
-    units = max(1, num_seqs) * num_kv_heads * _kv4_head_tiles(num_heads, num_kv_heads)
-    return KV4Scratch(torch.empty(_kv4_partial_floats(head_dim, sms), dtype=torch.float32, device=device),
-                      torch.zeros(units, dtype=torch.int32, device=device))
-
-
-def _kv4_partial_floats(head_dim: int, sms: int) -> int:
-    return 2 * sms * 16 * (head_dim + 2)
+    # two partial results per block; at most 48 heads in the blocks that an SM holds
+    floats = 2 * sms * 48 * (32 * -(-head_dim // 32) + 2)
+    counters = max(1, num_seqs) * num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
+    return KV4Scratch(num_seqs, (num_heads, num_kv_heads, head_dim), sms, torch.empty(floats, dtype=torch.float32, device=device),
+                      torch.zeros(counters, dtype=torch.int32, device=device))
 
 
 def _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window):
@@ -2347,7 +2343,7 @@ def _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_k
     _code(q, op)
     for name, t in (("q", q), ("out", out)):
         _kv4_rows(op, name, t, q.shape[0], num_heads * head_dim, q.dtype)
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.shape[1] < 1:
         raise ShapeError(op, "block_tables must be contiguous int32 [S, max_pages]")
     if block_tables.shape[0] < num_seqs:
         raise ShapeError(op, f"block_tables has {block_tables.shape[0]} rows for {num_seqs} requests")
@@ -2370,16 +2366,22 @@ def attn_decode_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     _kv4_attn_checks(op, q, out, cache, block_tables, S, num_heads, num_kv_heads, head_dim, window)
     _cuda(op, q, positions, scratch.partials, scratch.arrived)
     _int32_vec(positions, S, op, "positions")
-    tiles = _kv4_head_tiles(num_heads, num_kv_heads)
-    sms = torch.cuda.get_device_properties(q.device).multi_processor_count
-    need = _kv4_partial_floats(head_dim, sms)
-    if scratch.partials.numel() < need or scratch.arrived.numel() < S * num_kv_heads * tiles:
-        raise ShapeError(op, f"the scratch is too small: made for {scratch.arrived.numel()} of {S * num_kv_heads * tiles} counters and "
-                             f"{scratch.partials.numel()} of {need} floats (see kv4_scratch)")
-    splits = max(1, min(32, 2 * sms // max(1, S * num_kv_heads * tiles)))
+    if scratch.sizes != (num_heads, num_kv_heads, head_dim) or S > scratch.num_seqs:
+        raise ShapeError(op, f"the scratch was made for {scratch.num_seqs} requests of {scratch.sizes}, not for {S} of "
+                             f"{(num_heads, num_kv_heads, head_dim)} (heads, kv heads, head size)")
+    sms, code = scratch.sms, _code(q, op)
+    if code == 1 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0:
+        f = _fn("kv4_decode", "vob_kv4_decode", [_P, _L, _P, _L, _P, _L, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P, _L, _I, _P, _P])
+        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
+                 _ptr(positions), S, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), _ptr(scratch.partials),
+                 scratch.partials.numel(), _ptr(scratch.arrived), scratch.arrived.numel(), sms, _ptr(_scratch_for(q.device).err), _stream()),
+               op, 1 if S else 0)
+        return
+    # 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address
+    splits = max(1, min(32, 2 * sms // max(1, S * num_kv_heads * -(-(num_heads // num_kv_heads) // 16))))
     f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
     _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
-             _ptr(positions), _P(0), _P(0), S, 1, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), _code(q, op),
+             _ptr(positions), _P(0), _P(0), S, 1, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), code,
              splits, _ptr(scratch.partials), _ptr(scratch.arrived), _stream()), op, 1 if S else 0)
 
 
