@@ -13,6 +13,13 @@ BF16, F32 = torch.bfloat16, torch.float32
 HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}            # half a step, relative to the value
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    from vllm_oxide_b200 import kernels
+    kernels.gemm_sm100_check()
+
+
 def freq(hd, base=500000.0):
     return torch.tensor([base ** (-2.0 * i / hd) for i in range(hd // 2)], dtype=F32)
 

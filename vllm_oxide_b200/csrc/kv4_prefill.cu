@@ -1,0 +1,450 @@
+// Attention of portions of prompts over the 4-bit cache (layout: kv4.cuh) on the 5th-generation tensor cores: bfloat16 activations, head sizes
+// up to 128, any window, any page size, up to 128 heads per kv head.
+//
+// Math: s_j = scale q . K_j over the keys a row sees, softmax in float32 with a running maximum, out = sum_j softmax_j V_j, with
+// K_j = m + s n in bfloat16 (a code n in 0 .. 15 is exact in bfloat16, and m + s n is rounded once, 2^-8 of it), P in bfloat16. A row has
+// dozens to thousands of keys that share a tile's conversion, so here the codes become numbers once per tile and not scores once per row.
+//
+// One block: two tiles of 128 rows (token, head of the group) of one request and kv head, over tiles of 128 keys that both share:
+//   * four warps make the numbers: a thread takes a key, its codes already in registers (fetched a tile ahead straight from the
+//     pages, 128 contiguous bytes per eight keys), and writes K and V as bfloat16 into the swizzled operand tiles: per 8 codes 3 shifts,
+//     4 and-ors (a code in the low mantissa bits of 128 is 128 + n), 4 subtractions, 4 FMAs and one 16-byte store. The pairs that this gives are numbers
+//     (0,4), (1,5), (2,6), (3,7) of every eight; they stay in that order in the tiles, q is laid out likewise and the sums are put back at the end;
+//   * one thread issues S = Q K^T and O += P V (tcgen05.mma; S, P and O in tensor memory: S0 128 | S1 128 | O0 | O1 columns, P over its S);
+//   * two times four warps, a row a thread, do the softmax of the two row tiles: while one tile's rows work the tensor cores
+//     work for the other. P goes back in two halves, the first product starting on the first.
+// The running maximum moves only where a tile's exceeds it by more than 2^8 (sums, P and O share the reference), so O is rescaled rarely.
+// A key that is not finite is seen as NaN by the rows that see it, and by no other; its value is 0 in the tile.
+//
+// Every wait is bounded (sm100.cuh); on expiry the block raises the error flag, frees its tensor memory and returns.
+#include "kv4.cuh"
+VOB_PDL_SWITCH(kv4_prefill)
+#include "sm100.cuh"
+
+namespace {
+using namespace vob_kv4;
+using namespace vob_sm100;
+
+constexpr int BM = 128, BN = 128;                     // rows of a row tile, keys of a key tile
+// Four warpgroups: softmax of the row tiles (2), codes to numbers, issue of products (one thread). The registers that a block of 512 threads is
+// launched with, 128 each, are shared out anew: 2 x 176 + 80 + 80 = 4 x 128.
+constexpr int NTHREADS = 512;
+constexpr int REGS_ROWS = 176, REGS_CODES = 80, REGS_ISSUE = 80;
+static_assert(2 * REGS_ROWS + REGS_CODES + REGS_ISSUE == 4 * 128, "no more than the launch's registers");
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr int SPAN = 128 * 128;                       // bytes of 128 rows of 64 bfloat16
+
+struct Args {
+    const __nv_bfloat16* q;
+    long long q_stride;
+    __nv_bfloat16* out;
+    long long out_stride;
+    const unsigned char* cache;
+    const int* tables;
+    const int* seq_starts;
+    const int* context_lens;
+    int* err;
+    int max_pages, num_pages, H, G, hd, page_size, window;
+    float scale_log2;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// Eight codes -> m + s n as bfloat16, in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ uint4 numbers(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 m) {
+    const __nv_bfloat162 off = __floats2bfloat162_rn(128.f, 128.f);
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 x = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), off), s, m);
+        r[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int HD> constexpr size_t smem_bytes() { return 1024 + (size_t)(2 + 2 + 2) * (HD / 64) * SPAN + 256; }
+
+template <int HD>
+__global__ void __launch_bounds__(NTHREADS, 1)
+kv4_prefill_kernel(const Args a) {
+    constexpr int NS = HD / 64;                                        // spans of 64 numbers
+    constexpr int TILE = NS * SPAN;                                    // bytes of 128 rows of an operand
+    pdl_launch_dependents();
+    const int group = a.H / a.G, kvh = blockIdx.x, seq = blockIdx.y;
+    const int row0 = a.seq_starts[seq];
+    const int total_rows = (a.seq_starts[seq + 1] - row0) * group;
+    const int tile_rows = BM / group * group;                          // whole tokens only
+    const int first_row = (int)(gridDim.z - 1 - blockIdx.z) * 2 * tile_rows;      // later rows, which see more keys, start first
+    if (first_row >= total_rows) return;
+    const int ctx = a.context_lens[seq];
+
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* sQ = base;                                          // [2 row tiles]
+    unsigned char* sK = sQ + 2 * TILE;                                 // [2 stages]
+    unsigned char* sV = sK + 2 * TILE;                                 // [2 stages]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * TILE);
+    uint64_t* q_ready = bars;                // [2] a row tile's Q is in shared memory
+    uint64_t* k_full = bars + 2;             // [2] 128 threads have written the stage
+    uint64_t* v_full = bars + 4;             // [2]
+    uint64_t* k_free = bars + 6;             // [2] the products that read the stage are done
+    uint64_t* v_free = bars + 8;             // [2]
+    uint64_t* s_full = bars + 10;            // [2] a row tile's scores are there
+    uint64_t* p_first = bars + 12;           // [2] its 128 rows have written P of the tile's first 64 keys
+    uint64_t* p_second = bars + 14;          // [2] and of the others
+    uint64_t* o_full = bars + 16;            // [2] its O holds the tile
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // key tiles [from[t], to[t]) of each row tile
+    int from[2], to[2], hi = 0, lo = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r0 = first_row + t * tile_rows, r1 = min(total_rows, r0 + tile_rows);
+        from[t] = to[t] = 0;
+        if (r0 < r1) {
+            const int h = ctx + (r1 - 1) / group + 1, l = a.window ? max(0, ctx + r0 / group - a.window + 1) : 0;
+            from[t] = l / BN;
+            to[t] = (h + BN - 1) / BN;
+            hi = max(hi, h);
+            lo = min(lo, l);
+        }
+    }
+    const int j0 = from[0], j1 = max(to[0], to[1]);                    // the first tile has rows, and sees the earliest keys
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(q_ready + i, 128);
+            mbar_init(k_full + i, 128);
+            mbar_init(v_full + i, 128);
+            mbar_init(k_free + i, 1);
+            mbar_init(v_free + i, 1);
+            mbar_init(s_full + i, 1);
+            mbar_init(p_first + i, 128);
+            mbar_init(p_second + i, 128);
+            mbar_init(o_full + i, 1);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    pdl_wait(34);
+
+    if (warp >= 12) {
+        // ------------------------------------------------------------------ products
+        regs_down<REGS_ISSUE>();
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t idesc_qk = umma_idesc_bf16(BM, BN, false), idesc_pv = umma_idesc_bf16(BM, HD, true);
+            bool ok = true;
+            auto issue_qk = [&](int t, int j) {
+                const int s = (j - j0) & 1;
+                ok = ok && mbar_wait(q_ready + t, 0, abort_flag, a.err, 41) && mbar_wait(k_full + s, ((j - j0) >> 1) & 1, abort_flag, a.err, 42);
+                if (!ok) return;
+                tcgen05_fence_after();
+#pragma unroll
+                for (int h = 0; h < NS; ++h) {
+                    const uint64_t qd = umma_desc_sw128(sQ + t * TILE + h * SPAN), kd = umma_desc_sw128(sK + s * TILE + h * SPAN);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * BN, qd + 2 * k, kd + 2 * k, idesc_qk, (h > 0 || k > 0) ? 1u : 0u);
+                }
+                umma_commit(s_full + t);
+            };
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (from[t] == j0 && to[t] > j0) issue_qk(t, j0);
+            if (ok) umma_commit(k_free);
+            for (int j = j0; j < j1 && ok; ++j) {
+                const int s = (j - j0) & 1;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (j >= from[t] && j < to[t]) {
+                        const int n = j - from[t];
+                        const uint64_t vd = umma_desc_sw128(sV + s * TILE, SPAN);
+                        const uint32_t tO = tmem + 2 * BN + t * HD, tP = tmem + t * BN;
+                        ok = ok && mbar_wait(v_full + s, ((j - j0) >> 1) & 1, abort_flag, a.err, 43) &&
+                             mbar_wait(p_first + t, n & 1, abort_flag, a.err, 44);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_bf16_ts(tO, tP + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, (n > 0 || k > 0) ? 1u : 0u);
+                        ok = mbar_wait(p_second + t, n & 1, abort_flag, a.err, 45);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (int k = 4; k < 8; ++k) umma_bf16_ts(tO, tP + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, 1u);
+                        umma_commit(o_full + t);
+                    }
+                    if (j + 1 >= from[t] && j + 1 < to[t]) issue_qk(t, j + 1);
+                }
+                if (ok) {
+                    umma_commit(v_free + s);
+                    umma_commit(k_free + (s ^ 1));
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ------------------------------------------------------------------ codes to numbers
+        regs_down<REGS_CODES>();
+        const int i = threadIdx.x - 256;                                 // the thread's key of every tile
+        const int NC = chunks(a.hd), width = token_bytes(a.hd);
+        const int* bt = a.tables + (size_t)seq * a.max_pages;
+        auto page_of = [&](int j) {                                      // -2: no row sees the key; -1: behind the table
+            const int key = j * BN + i;
+            if (j >= j1 || key >= hi || key < lo) return -2;
+            const int idx = key / a.page_size;
+            return idx < a.max_pages ? bt[idx] : -1;
+        };
+        auto group_of = [&](int j, int page) -> const unsigned char* {
+            if (page < 0 || page >= a.num_pages) return nullptr;
+            const int key = j * BN + i, off = key % a.page_size;
+            return a.cache + group_at(page, kvh, off, a.G, a.page_size, width);
+        };
+        uint4 kr[HD / 32], vr[HD / 32];
+        uint2 par = make_uint2(0, 0);
+        auto load = [&](uint4 (&r)[HD / 32], const unsigned char* grp, int from_chunk) {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                r[c] = make_uint4(0, 0, 0, 0);
+                if (grp && c < NC) r[c] = *reinterpret_cast<const uint4*>(grp + (from_chunk + c) * 128 + (i & 7) * 16);
+            }
+        };
+        // tile key i of a page starts its group at a multiple of 8 keys, so (key & 7) == (i & 7)
+        int page = page_of(j0), next = page_of(j0 + 1);
+        const unsigned char* grp = group_of(j0, page);
+        load(kr, grp, 0);
+        load(vr, grp, NC);
+        if (grp) par = *reinterpret_cast<const uint2*>(grp + 256 * NC + 8 * (i & 7));
+        bool ok = true;
+        for (int j = j0; j < j1 && ok; ++j) {
+            const int s = (j - j0) & 1;
+            const uint32_t ph = ((j - j0) >> 1) & 1;
+            float2 ks = make_float2(0.f, 0.f), vs = ks;
+            if (grp) attend_scales(par, ks, vs);
+            else if (page != -2) ks = make_float2(NAN, NAN);             // a page outside the pool
+            const int page1 = next;
+            next = page_of(j + 2);
+            const unsigned char* grp1 = group_of(j + 1, page1);
+            par = make_uint2(0, 0);
+            if (grp1) par = *reinterpret_cast<const uint2*>(grp1 + 256 * NC + 8 * (i & 7));
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                // K, then V; a stage is free once the products of the tile before the last are done
+                ok = ok && mbar_wait((w ? v_free : k_free) + s, ph ^ 1, abort_flag, a.err, w ? 47 : 46);
+                if (!ok) break;
+                const float2 sm = w ? vs : ks;
+                const __nv_bfloat162 s2 = __float2bfloat162_rn(sm.x), m2 = __float2bfloat162_rn(sm.y);
+                unsigned char* row = (w ? sV : sK) + s * TILE + i * 128;
+                uint4(&r)[HD / 32] = w ? vr : kr;
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    const uint32_t code[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int piece = 4 * (c & 1) + u;               // 16 bytes of the row's 128, swizzled by the row
+                        *reinterpret_cast<uint4*>(row + (c >> 1) * SPAN + ((piece ^ (i & 7)) << 4)) = numbers(code[u], s2, m2);
+                    }
+                }
+                load(r, grp1, w * NC);                                   // a tile ahead
+                fence_proxy_async_smem();
+                mbar_arrive((w ? v_full : k_full) + s);
+            }
+            page = page1;
+            grp = grp1;
+        }
+    } else {
+        // ------------------------------------------------------------------ softmax rows
+        regs_up<REGS_ROWS>();
+        const int t = warp >> 2, quad = warp & 3;
+        const int t_from = t ? from[1] : from[0], t_to = t ? to[1] : to[0];
+        const int r = quad * 32 + lane;                                  // row of the tile = lane of tensor memory
+        const int rr = first_row + t * tile_rows + r;
+        const bool valid = r < tile_rows && rr < total_rows;
+        const int pos = valid ? ctx + rr / group : -1;
+        const int first_pos = ctx + (first_row + t * tile_rows) / group;
+        const int last_pos = ctx + (min(total_rows, first_row + (t + 1) * tile_rows) - 1) / group;
+        const long long at = (long long)(row0 + rr / group);
+        const int head = kvh * group + rr % group;
+        if (t_to > t_from) {
+            // Q: numbers (0,4), (1,5), (2,6), (3,7) of every eight, as the keys' tiles have them
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + at * a.q_stride + (size_t)head * a.hd);
+            unsigned char* row = sQ + t * TILE + r * 128;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (valid && 8 * c < a.hd) x = src[c];
+                const uint4 y = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
+                                           __byte_perm(x.y, x.w, 0x7632));
+                *reinterpret_cast<uint4*>(row + (c >> 3) * SPAN + (((c & 7) ^ (r & 7)) << 4)) = y;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_ready + t);
+        }
+        const uint32_t lane_at = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t tS = lane_at + t * BN, tO = lane_at + 2 * BN + t * HD;
+        float m_ref = -INFINITY, l = 0.f;
+        bool ok = true;
+        auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // tcgen05.ld / st are warp-wide: a warp gives up as a whole
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.err, code) ? 1 : 0) != 0;
+        };
+        for (int j = t_from; j < t_to && ok; ++j) {
+            const int n = j - t_from, kbase = j * BN;
+            const bool masked = kbase + BN - 1 > first_pos || (a.window && kbase <= last_pos - a.window);
+            const int see_from = a.window ? pos - a.window + 1 - kbase : -0x7fffffff, see_to = pos - kbase;      // keys of the tile that the row sees
+            if (!wait_all(s_full + t, n & 1, 48)) { ok = false; break; }
+            tcgen05_fence_after();
+            uint32_t va[32], vb[32];
+            auto scores = [&](int half) {
+                tmem_ld32(tS + 64 * half, va);
+                tmem_ld32(tS + 64 * half + 32, vb);
+                tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int k = 64 * half + i;
+                        if (k > see_to || k < see_from) va[i] = 0xff800000u;             // -inf
+                        if (k + 32 > see_to || k + 32 < see_from) vb[i] = 0xff800000u;
+                    }
+                }
+            };
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int half = 1; half >= 0; --half) {
+                scores(half);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    mx0 = max3(mx0, __uint_as_float(va[i]), __uint_as_float(vb[i]));
+                    mx1 = max3(mx1, __uint_as_float(va[i + 1]), __uint_as_float(vb[i + 1]));
+                }
+            }
+            const float mx2 = fmaxf(mx0, mx1) * a.scale_log2;            // scale > 0: the maximum commutes
+            const bool grow = mx2 > m_ref + 8.f;                         // also the first finite maximum
+            const float m_new = grow ? mx2 : m_ref;
+            const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.f;   // m_ref = -inf: 0
+            m_ref = m_new;
+            l *= alpha;
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            if (n > 0 && __any_sync(0xffffffffu, grow)) {
+                if (!wait_all(o_full + t, (n - 1) & 1, 49)) { ok = false; break; }
+                tcgen05_fence_after();
+#pragma unroll
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(tO + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                    tmem_st16(tO + c, v);
+                }
+            }
+            const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_use, -m_use);
+            float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (half) scores(1);
+                auto weigh = [&](const uint32_t (&v)[32], float2& acc, uint32_t to_column) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
+                        const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        acc = __fadd2_rn(acc, p);
+                        pk[i >> 1] = pack_bf16(p.x, p.y);
+                    }
+                    tmem_st16(tS + to_column, pk);                        // over scores that are in registers or done with
+                };
+                weigh(va, acc0, 32 * half);
+                weigh(vb, acc1, 32 * half + 16);
+                tmem_wait_st();
+                tcgen05_fence_before();
+                mbar_arrive((half ? p_second : p_first) + t);
+            }
+            l += (acc0.x + acc0.y) + (acc1.x + acc1.y);
+        }
+        if (ok && t_to > t_from && wait_all(o_full + t, (t_to - t_from - 1) & 1, 50)) {
+            tcgen05_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            __nv_bfloat16* dst = a.out + at * a.out_stride + (size_t)head * a.hd;
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(tO + c, v);
+                tmem_wait_ld();
+                if (valid && c < a.hd) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        // columns hold numbers 0 4 1 5 2 6 3 7
+                        uint4 x;
+                        x.x = pack_bf16(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 2]) * inv);
+                        x.y = pack_bf16(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 6]) * inv);
+                        x.z = pack_bf16(__uint_as_float(v[e + 1]) * inv, __uint_as_float(v[e + 3]) * inv);
+                        x.w = pack_bf16(__uint_as_float(v[e + 5]) * inv, __uint_as_float(v[e + 7]) * inv);
+                        *reinterpret_cast<uint4*>(dst + c + e) = x;
+                    }
+                }
+            }
+        }
+        tcgen05_fence_before();
+    }
+    __syncthreads();
+    if (warp == 12) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int HD> int launch(const Args& a, int S, long long row_tiles, cudaStream_t stream) {
+    static char done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(kv4_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<HD>());
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) done[dev] = 1;
+    }
+    return vob_launch(kv4_prefill_kernel<HD>, dim3(a.G, S, (unsigned)row_tiles), dim3(NTHREADS), smem_bytes<HD>(), stream, a);
+}
+
+}  // namespace
+
+// q [T, H * hd] bfloat16, out likewise (rows 16-byte aligned); seq_starts int32 [S + 1], context_lens int32 [S]; max_new = the longest portion.
+VOB_EXPORT int vob_kv4_prefill(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, long long num_pages,
+                               const int* tables, int max_pages, const int* seq_starts, const int* context_lens, int S, int max_new, int H, int G,
+                               int hd, int page_size, float scale, int window, int* err, cudaStream_t stream) {
+    if (S <= 0 || max_new <= 0) return 0;
+    if (H <= 0 || G <= 0 || H % G || hd <= 0 || hd % 16 || page_size <= 0 || page_size % 8 || num_pages <= 0 || num_pages > 0x7fffffffLL ||
+        max_pages <= 0 || window < 0 || !(scale > 0.f))
+        return VOB_ERR_BAD_ARG;
+    if (((uintptr_t)q & 15) || q_stride % 8 || ((uintptr_t)out & 15) || out_stride % 8 || ((uintptr_t)cache & 15)) return VOB_ERR_BAD_ARG;
+    const int group = H / G;
+    if (hd > 128 || group > BM || S > 65535) return VOB_ERR_UNSUPPORTED;
+    const long long tokens = 2 * (BM / group), row_tiles = ((long long)max_new + tokens - 1) / tokens;
+    if (row_tiles > 65535) return VOB_ERR_UNSUPPORTED;
+    const Args a = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache, tables, seq_starts, context_lens, err,
+                    max_pages, (int)num_pages, H, G, hd, page_size, window, scale * 1.4426950408889634f};
+    return hd <= 64 ? launch<64>(a, S, row_tiles, stream) : launch<128>(a, S, row_tiles, stream);
+}

@@ -91,7 +91,7 @@ def _int32_vec(t: torch.Tensor, n: int, op: str, name: str) -> None:
 
 _fn_cache = {}
 _MODULES = ("elementwise", "gemm_f32", "gemm_sm100", "gemm_sm100_pair", "attention", "attention_mma", "attention_sm100", "sampling",
-            "streams", "recurrence", "latent_attention", "attention_flex", "moe", "kv4", "kv4_decode")
+            "streams", "recurrence", "latent_attention", "attention_flex", "moe", "kv4", "kv4_decode", "kv4_prefill")
 
 # Per-op device timing, off unless a profile is being taken: CUDA events around each wrapper
 # (the reference times ops by wall clock on the CPU and notes that a CUDA backend must use
@@ -924,7 +924,7 @@ def gemm_sm100_check() -> None:
             sc.err.zero_()
             raise KernelError(f"a bounded wait expired inside a tensor-core kernel (code {code}: 1-4 = matrix product: TMA "
                               "producer, MMA issuer, epilogue, peers of a split; 11-21 = attention: 11-12 TMA producer, 13-17 MMA issuer, "
-                              "18-21 softmax rows; 31 = decode attention over a 4-bit cache); its result is not valid")
+                              "18-21 softmax rows; 31 = decode attention over a 4-bit cache, 41-50 = portions over it); its result is not valid")
 
 
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None, fixed_w: bool = False) -> None:
@@ -2398,6 +2398,14 @@ def attn_prefill_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, bl
     _cuda(op, q, seq_starts, context_lens)
     _int32_vec(seq_starts, num_seqs + 1, op, "seq_starts")
     _int32_vec(context_lens, num_seqs, op, "context_lens")
+    if (_code(q, op) == 1 and head_dim <= 128 and num_heads // num_kv_heads <= 128 and scale > 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+            and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0):
+        f = _fn("kv4_prefill", "vob_kv4_prefill", [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P])
+        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
+                 _ptr(seq_starts), _ptr(context_lens), num_seqs, max_new, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale),
+                 int(window), _ptr(_scratch_for(q.device).err), _stream()), op, 1 if num_seqs > 0 and max_new > 0 else 0)
+        return
+    # 32-bit arithmetic: the float32 engine, larger heads, and rows that the tensor-core kernel cannot address
     f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
     _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
              _P(0), _ptr(seq_starts), _ptr(context_lens), num_seqs, max_new, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale),
