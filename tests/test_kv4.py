@@ -109,3 +109,18 @@ def test_scratch_refuses(no_gpu):
     for bad in ((-1, 4, 2, 32), (1, 3, 2, 32), (1, 4, 2, 24), (1, 4, 0, 32)):
         with pytest.raises(ShapeError):
             kernels.kv4_scratch(*bad, "cpu")
+
+
+def test_engine_config_takes_four_or_none():
+    from vllm_oxide_b200.config import EngineConfig
+    from vllm_oxide_b200.errors import ConfigError
+    assert EngineConfig().cache_bits is None and EngineConfig(cache_bits=4).cache_bits == 4
+    for bad in (3, 8, 16, "4", 4.5, 4.0, True, 0):
+        with pytest.raises(ConfigError, match="cache_bits"):
+            EngineConfig(cache_bits=bad)
+
+
+def test_architectures_say_what_they_cache():
+    from vllm_oxide_b200 import models  # noqa: F401
+    from vllm_oxide_b200.config import architecture_for, known_architectures
+    assert [a for a in known_architectures() if 4 in architecture_for({"architectures": [a]}).cache_bits] == ["LlamaForCausalLM"]

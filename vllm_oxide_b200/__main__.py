@@ -24,6 +24,7 @@ import time
 
 def _engine_args(ap):
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-bits", type=int, default=None, help="4: cached keys and values in 4 bits (default: in the compute dtype)")
     ap.add_argument("--max-batch-tokens", type=int, default=2048)
     ap.add_argument("--max-seqs", type=int, default=32)
     ap.add_argument("--max-model-len", type=int, default=8192)
@@ -37,7 +38,7 @@ def _engine_args(ap):
 def _engine_kwargs(a):
     return dict(max_batch_tokens=a.max_batch_tokens, max_seqs=a.max_seqs, max_model_len=a.max_model_len,
                 block_size=a.block_size, kv_pool_bytes=a.kv_pool_bytes, num_pages=a.num_pages,
-                prefill_chunk=a.prefill_chunk, cuda_graphs=not a.no_cuda_graphs)
+                prefill_chunk=a.prefill_chunk, cuda_graphs=not a.no_cuda_graphs, cache_bits=a.cache_bits)
 
 
 def cmd_generate(argv):

@@ -3,7 +3,7 @@
 The five knobs and their defaults are the reference's `EngineConfig`
 (crates/engine/src/model.rs:37-66): max_batch_tokens 2048, max_seqs 32,
 max_model_len 8192, block_size 16, kv_pool_bytes 2 GiB. Added here: the compute
-dtype, an explicit page count (tests want tiny pools), the largest portion of a
+dtype, the bits that cached keys and values are held in, an explicit page count (tests want tiny pools), the largest portion of a
 prompt that one step takes, whether decode steps replay CUDA graphs, and the switches of
 what makes a decode step fast (programmatic dependent launch, folded norms, running one
 step ahead of the host's reads).
@@ -43,6 +43,7 @@ class EngineConfig:
     kv_pool_bytes: int = 2 << 30       # cache budget when num_pages is not given
     num_pages: Optional[int] = None    # explicit page count per cache group
     dtype: torch.dtype = torch.bfloat16
+    cache_bits: Optional[int] = None   # 4: keys and values are cached in 4 bits (some 0.27 of bfloat16's bytes; architectures that name it); None: as dtype
     prefill_chunk: Optional[int] = None  # most prompt tokens of one request per step
     admission_watermark_pages: int = 0   # while others run, admit a request only if so many pages stay free behind
                                          # its first portion (0: whenever a token fits)
@@ -63,6 +64,8 @@ class EngineConfig:
                 raise ConfigError(f"engine config: {k} must be a positive integer, got {v!r}")
         if self.block_size % 8 != 0:
             raise ConfigError(f"engine config: block_size must be a multiple of 8, got {self.block_size}")
+        if self.cache_bits is not None and (not isinstance(self.cache_bits, int) or self.cache_bits != 4):
+            raise ConfigError(f"engine config: cache_bits must be 4 or None (the compute dtype), got {self.cache_bits!r}")
         if self.num_pages is not None and self.num_pages <= 0:
             raise ConfigError("engine config: num_pages must be positive")
         if self.prefill_chunk is not None and self.prefill_chunk <= 0:

@@ -8,7 +8,7 @@ builder that turns (configuration, weights) into a `ModelSpec` of parts. Unknown
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Callable, Dict
+from typing import Callable, Dict, Tuple
 
 from ..errors import ConfigError
 
@@ -19,6 +19,7 @@ class Architecture:
     config_cls: type                 # has from_dict(dict, where) and to_dict()
     manifest: Callable               # manifest(config) -> {tensor name: TensorSpec}
     build: Callable                  # build(config, weights: WeightSet, ctx: BuildContext) -> ModelSpec
+    cache_bits: Tuple[int, ...] = ()   # what `EngineConfig.cache_bits` may be beside None: the builder passes it on to its mixers
 
 
 _REGISTRY: Dict[str, Architecture] = {}

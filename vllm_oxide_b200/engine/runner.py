@@ -25,7 +25,7 @@ from .. import kernels
 from ..cache.pools import EMBEDDING_STATE, CachePools
 from ..config import EngineConfig, architecture_for, read_config_json
 from ..csrc.build import runtime_module
-from ..errors import CapacityError, KernelError, ShapeError
+from ..errors import CapacityError, ConfigError, KernelError, ShapeError
 from ..tuning import TUNING
 from ..parts.attention import decode_balance
 from ..parts.base import ModelSpec, StepContext, Workspace, aligned
@@ -89,13 +89,18 @@ class ModelRunner:
         self.dtype = engine.dtype
         torch.cuda.set_device(self.device)
         arch = arch or architecture_for(config.to_dict())
+        if engine.cache_bits is not None and engine.cache_bits not in arch.cache_bits:
+            raise ConfigError(f"architecture {arch.name!r} does not cache keys and values in {engine.cache_bits} bits")
         manifest = arch.manifest(config)
         if isinstance(tensors_or_dir, (str, os.PathLike)):
             weights = load_safetensors_weights(str(tensors_or_dir), manifest, device=self.device)
         else:
             weights = weights_from_tensors(tensors_or_dir, manifest)
         kernels.set_pdl(bool(engine.pdl))
-        self.spec: ModelSpec = arch.build(config, weights, BuildContext(dtype=self.dtype, device=self.device))
+        build = BuildContext(dtype=self.dtype, device=self.device)
+        if engine.cache_bits is not None:
+            build.cache_bits, build.max_seqs = engine.cache_bits, engine.max_seqs
+        self.spec: ModelSpec = arch.build(config, weights, build)
         del weights
         if self.dtype == torch.bfloat16:
             # the library product (many rows) must add its split-K partial sums in float32 too

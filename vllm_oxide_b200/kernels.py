@@ -2257,6 +2257,8 @@ def _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim):
         raise ShapeError(op, f"{cache.shape[0]} pages of {cache.shape[2]} tokens are beyond 2^31 - 1 slots")
     if cache.data_ptr() % 16:
         raise ShapeError(op, "the cache must start on a 16-byte boundary")
+    if cache.is_cuda and cache.device.index != torch.cuda.current_device():
+        raise ShapeError(op, f"the tensors are on {cache.device}, the current device is cuda:{torch.cuda.current_device()}: launches go to its stream")
     if not kv4_supported(num_heads, num_kv_heads, head_dim, cache.shape[2]):
         raise ShapeError(op, f"sizes not supported: heads {num_heads}/{num_kv_heads}, head_dim {head_dim} (multiples of 16 up to 256), "
                              f"page {cache.shape[2]} (multiples of 8)")

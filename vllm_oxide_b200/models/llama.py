@@ -9,10 +9,11 @@ crates/engine/src/weights.rs:154-156).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict
+from typing import Dict, Optional
 
 import torch
 
+from .. import kernels
 from ..config.model_config import LlamaConfig
 from ..config.registry import Architecture, register_architecture
 from ..parts import (Attention, Block, Embedding, LayerCall, LMHead, ModelSpec, RMSNorm, Rotary, SwiGLU)
@@ -24,6 +25,8 @@ from ..weights.loader import TensorSpec, WeightSet
 class BuildContext:
     dtype: torch.dtype
     device: str
+    cache_bits: Optional[int] = None        # `EngineConfig.cache_bits`, where the architecture names it
+    max_seqs: int = 256                     # most requests in one step
 
 
 def llama_manifest(cfg: LlamaConfig) -> Dict[str, TensorSpec]:
@@ -52,13 +55,16 @@ def build_llama(cfg: LlamaConfig, weights: WeightSet, ctx: BuildContext) -> Mode
     dt, dev = ctx.dtype, ctx.device
     rotary = Rotary(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, dev)
     embedding = Embedding(weights.take("model.embed_tokens.weight"), dt, dev)
+    scratch = None
+    if ctx.cache_bits == 4:                 # one for all layers, which run one behind the other
+        scratch = kernels.kv4_scratch(ctx.max_seqs, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, dev)
     blocks, schedule = [], []
     for i in range(cfg.num_hidden_layers):
         p = f"model.layers.{i}."
         mixer = Attention(weights.take(p + "self_attn.q_proj.weight"), weights.take(p + "self_attn.k_proj.weight"),
                           weights.take(p + "self_attn.v_proj.weight"), weights.take(p + "self_attn.o_proj.weight"),
                           cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, position=rotary,
-                          dtype=dt, device=dev)
+                          dtype=dt, device=dev, cache_bits=ctx.cache_bits, kv4_scratch=scratch)
         ff = SwiGLU(weights.take(p + "mlp.gate_proj.weight"), weights.take(p + "mlp.up_proj.weight"),
                     weights.take(p + "mlp.down_proj.weight"), dt, dev)
         blocks.append(Block(RMSNorm(weights.take(p + "input_layernorm.weight"), cfg.rms_norm_eps, dev), mixer,
@@ -76,5 +82,5 @@ def build_llama(cfg: LlamaConfig, weights: WeightSet, ctx: BuildContext) -> Mode
                      max_position=cfg.max_position_embeddings, eos_token_ids=cfg.eos_token_ids, weight_bytes=wbytes)
 
 
-LLAMA = Architecture(name="LlamaForCausalLM", config_cls=LlamaConfig, manifest=llama_manifest, build=build_llama)
+LLAMA = Architecture(name="LlamaForCausalLM", config_cls=LlamaConfig, manifest=llama_manifest, build=build_llama, cache_bits=(4,))
 register_architecture(LLAMA, replace=True)

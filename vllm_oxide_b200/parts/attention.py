@@ -10,6 +10,10 @@ Parameters: head counts, head size, an optional window (the last `window` keys o
 optional score scale (default head_dim^-1/2, crates/engine/src/backend/cpu/attention.rs:91),
 and the position encoding (a `Rotary` or None). With `wk`/`wv` None the mixer writes no cache:
 it must be scheduled on a cache that another layer writes.
+
+With `cache_bits` 4 the cache holds keys and values in 4 bits with a scale and a minimum per vector (one uint8 tensor per layer, some
+0.27 of bfloat16's bytes; csrc/kv4.cuh): the append kernel rotates, quantises and writes behind the projection, and attention works on
+the codes (`kernels.attn_decode_kv4`, `kernels.attn_prefill_kv4`), in either compute dtype.
 """
 from __future__ import annotations
 
@@ -20,7 +24,7 @@ import torch
 
 from .. import kernels
 from ..tuning import TUNING
-from .base import CacheSpec, FoldedState, LayerCache, Mixer, StepContext, aligned
+from .base import CacheSpec, FoldedState, LayerCache, Mixer, PagedTensorSpec, StepContext, aligned
 from .linear import matmul, to_compute
 
 
@@ -84,12 +88,21 @@ def decode_scratch_blocks(kv_heads: int, num_sms: int) -> int:
 class Attention(Mixer):
     def __init__(self, wq: torch.Tensor, wk: Optional[torch.Tensor], wv: Optional[torch.Tensor], wo: torch.Tensor,
                  num_heads: int, num_kv_heads: int, head_dim: int, position=None, window: Optional[int] = None,
-                 scale: Optional[float] = None, dtype=torch.bfloat16, device="cuda"):
+                 scale: Optional[float] = None, dtype=torch.bfloat16, device="cuda", cache_bits: Optional[int] = None,
+                 kv4_scratch: Optional["kernels.KV4Scratch"] = None):
+        """`kv4_scratch` (with `cache_bits` 4): scratch of the decode kernel, which layers that run one behind the other may share
+        (default: one of its own, for at most 256 requests in a step)."""
         self.H, self.KV, self.hd = int(num_heads), int(num_kv_heads), int(head_dim)
         if self.H % self.KV != 0:
             raise ValueError(f"{self.H} heads are not a multiple of {self.KV} kv heads")
         if self.hd % 16 != 0 or self.hd > 256:
             raise ValueError(f"head_dim {self.hd} is not supported: multiples of 16 up to 256")
+        if cache_bits not in (None, 4):
+            raise ValueError(f"cache_bits {cache_bits!r}: 4 or None")
+        self.kv4 = cache_bits == 4
+        self.kv4_scratch = kv4_scratch
+        if self.kv4 and kv4_scratch is None:
+            self.kv4_scratch = kernels.kv4_scratch(256, self.H, self.KV, self.hd, device)
         hidden = wq.shape[1]
         if wq.shape != (self.H * self.hd, hidden) or wo.shape != (hidden, self.H * self.hd):
             raise ValueError(f"q/o projection shapes {list(wq.shape)} / {list(wo.shape)} do not fit "
@@ -119,6 +132,9 @@ class Attention(Mixer):
         self._arrived = None
 
     def cache_spec(self) -> Optional[CacheSpec]:
+        if self.kv4:
+            return CacheSpec(kind="window" if self.window else "full", window=self.window,
+                             tensors=(PagedTensorSpec(self.KV, kernels.kv4_width(self.hd), torch.uint8),))
         return CacheSpec(self.KV, self.hd, "window" if self.window else "full", self.window)
 
     def weight_bytes(self) -> int:
@@ -126,7 +142,7 @@ class Attention(Mixer):
 
     def _few_rows_path(self, rows: int) -> bool:
         """Steps of few rows: rotary positions and the cache write happen in the projection's epilogue."""
-        return (self.dtype == torch.bfloat16 and self.fused and self.owns_cache and rows <= TUNING.few_rows
+        return (self.dtype == torch.bfloat16 and self.fused and self.owns_cache and not self.kv4 and rows <= TUNING.few_rows
                 and kernels.gemm_qkv_rope_supported(self.hd) and self.hidden % 8 == 0)
 
     def workspace_bytes(self, rows: int) -> int:
@@ -136,9 +152,12 @@ class Attention(Mixer):
         return aligned(rows * q_cols * es) + aligned(rows * self.H * self.hd * es)
 
     def folded_workspace_bytes(self, rows: int) -> int:
-        return 2 * aligned(rows * self.H * self.hd * 2)
+        q_cols = self.w_qkv.shape[0] if self.kv4 else self.H * self.hd
+        return aligned(rows * q_cols * 2) + aligned(rows * self.H * self.hd * 2)
 
     def kernel_modules(self, dtype, max_rows):
+        if self.kv4:
+            return ("elementwise", "gemm_f32", "kv4") if dtype == torch.float32 else ("elementwise", "gemm_sm100", "kv4", "kv4_decode", "kv4_prefill")
         if dtype == torch.float32:
             return ("elementwise", "gemm_f32", "attention")
         mods = ["elementwise", "gemm_sm100", "attention"]
@@ -162,7 +181,9 @@ class Attention(Mixer):
             return matmul(attn, self.w_o, out if out is not None else ctx.alloc((T, self.hidden)))
         qkv = matmul(x, self.w_qkv, ctx.alloc((T, self.w_qkv.shape[0])))
         q = qkv[:, :qd]
-        if self.owns_cache and cache.write:
+        if self.owns_cache and cache.write and self.kv4:
+            self._append(qkv, ctx, cache)
+        elif self.owns_cache and cache.write:
             k, v = qkv[:, qd:qd + kd], qkv[:, qd + kd:]
             kernels.rope_kv_write(q, k, v, ctx.positions, ctx.slot_mapping[cache.group], inv_freq,
                                   cache.k, cache.v, self.H, self.KV, self.hd)
@@ -171,6 +192,12 @@ class Attention(Mixer):
         attn = ctx.alloc((T, qd))
         self.attend(q, attn, ctx, cache)
         return matmul(attn, self.w_o, out if out is not None else ctx.alloc((T, self.hidden)))
+
+    def _append(self, qkv: torch.Tensor, ctx: StepContext, cache: LayerCache) -> None:
+        """4-bit cache: q turns in place, k (turned) and v go to their slots."""
+        qd, kd = self.H * self.hd, self.KV * self.hd
+        kernels.kv4_append(qkv[:, :qd], qkv[:, qd:qd + kd], qkv[:, qd + kd:], ctx.positions, ctx.slot_mapping[cache.group],
+                           self.position.inv_freq if self.position is not None else None, cache.tensors[0], self.H, self.KV, self.hd)
 
     def can_fold(self) -> bool:
         """Whether this mixer can take its input in folded form (see FoldedState): bfloat16, its own
@@ -185,6 +212,14 @@ class Attention(Mixer):
         T = st.xn.shape[0]
         qd = self.H * self.hd
         inv_freq = self.position.inv_freq if self.position is not None else None
+        if self.kv4:
+            qkv = ctx.alloc((T, self.w_qkv.shape[0]))
+            kernels.gemm_fused(st.xn, self.w_qkv, qkv, kernels.EPI_STORE, self.w_qkv.shape[0], ssq_in=st.ssq, eps=eps)
+            self._append(qkv, ctx, cache)
+            attn = ctx.alloc((T, qd))
+            self.attend(qkv[:, :qd], attn, ctx, cache)
+            kernels.gemm_fused(attn, self.w_o, None, kernels.EPI_RESID, self.hidden, resid=(st.resid, next_w, st.xn, st.ssq))
+            return
         q = ctx.alloc((T, qd))
         kernels.gemm_fused(st.xn, self.w_qkv, q, kernels.EPI_QKV, self.w_qkv.shape[0], ssq_in=st.ssq, eps=eps,
                            qkv=(ctx.positions, ctx.slot_mapping[cache.group] if cache.write else None, inv_freq, cache.k, cache.v,
@@ -199,9 +234,19 @@ class Attention(Mixer):
         mma.sync portion kernel. In a mixed step the leading requests that bring one token each go
         to the decode kernel and the portions behind them to the portion kernel (a single token is
         a poor portion: one block would walk all its keys for four rows of a 128-row tile).
-        Otherwise (float32, other head sizes) the general kernel."""
+        Otherwise (float32, other head sizes) the general kernel. A 4-bit cache has kernels of its own for single tokens and
+        for portions, which a mixed step shares out in the same way."""
         page = cache.k.shape[2]
         bt = ctx.block_tables[cache.group]
+        if self.kv4:
+            lead = ctx.rows if ctx.decode_only else ctx.lead_single if self.split_mixed and ctx.lead_single < ctx.seqs else 0
+            if lead:
+                kernels.attn_decode_kv4(q[:lead], out[:lead], cache.k, bt, ctx.positions[:lead], self.H, self.KV, self.hd, self.scale,
+                                        self.window, scratch=self.kv4_scratch)
+            if not ctx.decode_only:
+                kernels.attn_prefill_kv4(q, out, cache.k, bt[lead:], ctx.seq_starts[lead:], ctx.context_lens[lead:], ctx.seqs - lead,
+                                         ctx.max_new or ctx.rows, self.H, self.KV, self.hd, self.scale, self.window)
+            return
         if self.dtype == torch.bfloat16 and self.impl != "general" and self.scale > 0:
             decode_ok = kernels.attn_mma_supported(self.H, self.KV, self.hd, page, True)
             if ctx.decode_only and decode_ok:
@@ -244,7 +289,7 @@ class Attention(Mixer):
 
     def balance_rule(self, page_size: int):
         """(kv heads, head size, SMs) for `decode_balance_rule`, or None where this mixer's single tokens never run balanced."""
-        if (self.dtype != torch.bfloat16 or self.impl == "general" or not self.scale > 0 or self.window
+        if (self.dtype != torch.bfloat16 or self.impl == "general" or not self.scale > 0 or self.window or self.kv4
                 or not kernels.attn_mma_supported(self.H, self.KV, self.hd, page_size, True)):
             return None
         return self.KV, self.hd, self.num_sms
