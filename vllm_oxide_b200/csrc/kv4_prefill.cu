@@ -6,7 +6,7 @@
 // dozens to thousands of keys that share a tile's conversion, so here the codes become numbers once per tile and not scores once per row.
 //
 // One block: two tiles of 128 rows (token, head of the group) of one request and kv head, over tiles of 128 keys that both share:
-//   * four warps make the numbers: a thread takes a key, its codes already in registers (fetched a tile ahead straight from the
+//   * four warps each make the numbers of K and of V: a thread takes a key, its codes already in registers (fetched a tile ahead straight from the
 //     pages, 128 contiguous bytes per eight keys), and writes K and V as bfloat16 into the swizzled operand tiles: per 8 codes 3 shifts,
 //     4 and-ors (a code in the low mantissa bits of 128 is 128 + n), 4 subtractions, 4 FMAs and one 16-byte store. The pairs that this gives are numbers
 //     (0,4), (1,5), (2,6), (3,7) of every eight; they stay in that order in the tiles, q is laid out likewise and the sums are put back at the end;
@@ -26,11 +26,11 @@ using namespace vob_kv4;
 using namespace vob_sm100;
 
 constexpr int BM = 128, BN = 128;                     // rows of a row tile, keys of a key tile
-// Four warpgroups: softmax of the row tiles (2), codes to numbers, issue of products (one thread). The registers that a block of 512 threads is
-// launched with, 128 each, are shared out anew: 2 x 176 + 80 + 80 = 4 x 128.
-constexpr int NTHREADS = 512;
-constexpr int REGS_ROWS = 176, REGS_CODES = 80, REGS_ISSUE = 80;
-static_assert(2 * REGS_ROWS + REGS_CODES + REGS_ISSUE == 4 * 128, "no more than the launch's registers");
+// Five warpgroups: softmax of the row tiles (2), codes to numbers of K and of V, issue of products (one thread). The registers that a block of 640
+// threads is launched with, 96 each, are shared out anew.
+constexpr int NTHREADS = 640;
+constexpr int REGS_ROWS = 136, REGS_CODES = 72, REGS_ISSUE = 64;
+static_assert(2 * REGS_ROWS + 2 * REGS_CODES + REGS_ISSUE == 5 * 96, "no more than the launch's registers");
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int SPAN = 128 * 128;                       // bytes of 128 rows of 64 bfloat16
@@ -47,8 +47,16 @@ struct Args {
     int* err;
     int max_pages, num_pages, H, G, hd, page_size, window;
     float scale_log2;
+    unsigned page_magic;         // ceil(2^32 / (page_size / 8)): the page of a group of eight keys without a division
 };
 
+// One lane of a converged warp, which the compiler then knows to be one thread: an instruction whose operands are uniform is issued as such. (With
+// `lane == 0` the 32 products of a key tile at head size 128 took 4,000 clocks to issue, with this 1,300.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -142,7 +150,7 @@ kv4_prefill_kernel(const Args a) {
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -152,10 +160,10 @@ kv4_prefill_kernel(const Args a) {
     const uint32_t tmem = *tmem_holder;
     pdl_wait(34);
 
-    if (warp >= 12) {
+    if (warp >= 16) {
         // ------------------------------------------------------------------ products
         regs_down<REGS_ISSUE>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 16 && elect_one()) {
             constexpr uint32_t idesc_qk = umma_idesc_bf16(BM, BN, false), idesc_pv = umma_idesc_bf16(BM, HD, true);
             bool ok = true;
             auto issue_qk = [&](int t, int j) {
@@ -171,16 +179,17 @@ kv4_prefill_kernel(const Args a) {
                 }
                 umma_commit(s_full + t);
             };
-#pragma unroll
+#pragma unroll 1
             for (int t = 0; t < 2; ++t)
-                if (from[t] == j0 && to[t] > j0) issue_qk(t, j0);
+                if ((t ? from[1] : from[0]) == j0 && (t ? to[1] : to[0]) > j0) issue_qk(t, j0);
             if (ok) umma_commit(k_free);
             for (int j = j0; j < j1 && ok; ++j) {
                 const int s = (j - j0) & 1;
-#pragma unroll
+#pragma unroll 1
                 for (int t = 0; t < 2; ++t) {
-                    if (j >= from[t] && j < to[t]) {
-                        const int n = j - from[t];
+                    const int t_from = t ? from[1] : from[0], t_to = t ? to[1] : to[0];
+                    if (j >= t_from && j < t_to) {
+                        const int n = j - t_from;
                         const uint64_t vd = umma_desc_sw128(sV + s * TILE, SPAN);
                         const uint32_t tO = tmem + 2 * BN + t * HD, tP = tmem + t * BN;
                         ok = ok && mbar_wait(v_full + s, ((j - j0) >> 1) & 1, abort_flag, a.err, 43) &&
@@ -197,7 +206,7 @@ kv4_prefill_kernel(const Args a) {
                         for (int k = 4; k < 8; ++k) umma_bf16_ts(tO, tP + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, 1u);
                         umma_commit(o_full + t);
                     }
-                    if (j + 1 >= from[t] && j + 1 < to[t]) issue_qk(t, j + 1);
+                    if (j + 1 >= t_from && j + 1 < t_to) issue_qk(t, j + 1);
                 }
                 if (ok) {
                     umma_commit(v_free + s);
@@ -207,73 +216,63 @@ kv4_prefill_kernel(const Args a) {
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // ------------------------------------------------------------------ codes to numbers
+        // ------------------------------------------------------------------ codes to numbers: K (warps 8 to 11), V (12 to 15)
         regs_down<REGS_CODES>();
-        const int i = threadIdx.x - 256;                                 // the thread's key of every tile
+        const int i = threadIdx.x & 127;                                 // the thread's key of every tile
+        const bool is_v = warp >= 12;
         const int NC = chunks(a.hd), width = token_bytes(a.hd);
         const int* bt = a.tables + (size_t)seq * a.max_pages;
+        unsigned char* tiles = is_v ? sV : sK;
+        uint64_t *full = is_v ? v_full : k_full, *free_ = is_v ? v_free : k_free;
+        // (a division takes the unit that the rows' exponentials keep busy)
+        auto page_index = [&](int key) { return (int)(a.page_magic ? __umulhi((unsigned)key >> 3, a.page_magic) : (unsigned)key >> 3); };
         auto page_of = [&](int j) {                                      // -2: no row sees the key; -1: behind the table
             const int key = j * BN + i;
             if (j >= j1 || key >= hi || key < lo) return -2;
-            const int idx = key / a.page_size;
+            const int idx = page_index(key);
             return idx < a.max_pages ? bt[idx] : -1;
         };
-        auto group_of = [&](int j, int page) -> const unsigned char* {
-            if (page < 0 || page >= a.num_pages) return nullptr;
-            const int key = j * BN + i, off = key % a.page_size;
-            return a.cache + group_at(page, kvh, off, a.G, a.page_size, width);
-        };
-        uint4 kr[HD / 32], vr[HD / 32];
-        uint2 par = make_uint2(0, 0);
-        auto load = [&](uint4 (&r)[HD / 32], const unsigned char* grp, int from_chunk) {
+        uint4 r[HD / 32];
+        uint2 par;
+        int page;
+        // codes, scales and minima of the thread's key of tile j, from its page `at`
+        auto load = [&](int j, int at) {
+            page = at;
+            const unsigned char* grp = nullptr;
+            if (at >= 0 && at < a.num_pages)                              // groups of eight begin at multiples of 8 keys: (key & 7) == (i & 7)
+                grp = a.cache + group_at(at, kvh, j * BN + i - page_index(j * BN + i) * a.page_size, a.G, a.page_size, width) + (i & 7) * 16;
+            else if (at >= 0) page = -1;                                  // a page outside the pool
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
                 r[c] = make_uint4(0, 0, 0, 0);
-                if (grp && c < NC) r[c] = *reinterpret_cast<const uint4*>(grp + (from_chunk + c) * 128 + (i & 7) * 16);
+                if (grp && c < NC) r[c] = *reinterpret_cast<const uint4*>(grp + ((is_v ? NC : 0) + c) * 128);
             }
-        };
-        // tile key i of a page starts its group at a multiple of 8 keys, so (key & 7) == (i & 7)
-        int page = page_of(j0), next = page_of(j0 + 1);
-        const unsigned char* grp = group_of(j0, page);
-        load(kr, grp, 0);
-        load(vr, grp, NC);
-        if (grp) par = *reinterpret_cast<const uint2*>(grp + 256 * NC + 8 * (i & 7));
-        bool ok = true;
-        for (int j = j0; j < j1 && ok; ++j) {
-            const int s = (j - j0) & 1;
-            const uint32_t ph = ((j - j0) >> 1) & 1;
-            float2 ks = make_float2(0.f, 0.f), vs = ks;
-            if (grp) attend_scales(par, ks, vs);
-            else if (page != -2) ks = make_float2(NAN, NAN);             // a page outside the pool
-            const int page1 = next;
-            next = page_of(j + 2);
-            const unsigned char* grp1 = group_of(j + 1, page1);
             par = make_uint2(0, 0);
-            if (grp1) par = *reinterpret_cast<const uint2*>(grp1 + 256 * NC + 8 * (i & 7));
+            if (grp) par = *reinterpret_cast<const uint2*>(grp + 256 * NC - (i & 7) * 8);
+        };
+        load(j0, page_of(j0));
+        int next = page_of(j0 + 1);
+        for (int j = j0; j < j1; ++j) {
+            const int s = (j - j0) & 1;
+            float2 ks = make_float2(0.f, 0.f), vs = ks;
+            if (page >= 0) attend_scales(par, ks, vs);
+            else if (page == -1) ks = make_float2(NAN, NAN);
+            const float2 sm = is_v ? vs : ks;
+            const __nv_bfloat162 s2 = __float2bfloat162_rn(sm.x), m2 = __float2bfloat162_rn(sm.y);
+            // a stage is free once the products of the tile before the last are done
+            if (!mbar_wait(free_ + s, (((j - j0) >> 1) & 1) ^ 1, abort_flag, a.err, 46)) break;
+            unsigned char* row = tiles + s * TILE + i * 128;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                // K, then V; a stage is free once the products of the tile before the last are done
-                ok = ok && mbar_wait((w ? v_free : k_free) + s, ph ^ 1, abort_flag, a.err, w ? 47 : 46);
-                if (!ok) break;
-                const float2 sm = w ? vs : ks;
-                const __nv_bfloat162 s2 = __float2bfloat162_rn(sm.x), m2 = __float2bfloat162_rn(sm.y);
-                unsigned char* row = (w ? sV : sK) + s * TILE + i * 128;
-                uint4(&r)[HD / 32] = w ? vr : kr;
+            for (int c = 0; c < HD / 32; ++c) {
+                const uint32_t code[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    const uint32_t code[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int piece = 4 * (c & 1) + u;               // 16 bytes of the row's 128, swizzled by the row
-                        *reinterpret_cast<uint4*>(row + (c >> 1) * SPAN + ((piece ^ (i & 7)) << 4)) = numbers(code[u], s2, m2);
-                    }
-                }
-                load(r, grp1, w * NC);                                   // a tile ahead
-                fence_proxy_async_smem();
-                mbar_arrive((w ? v_full : k_full) + s);
+                for (int u = 0; u < 4; ++u)                               // 16 bytes of the row's 128, swizzled by the row
+                    *reinterpret_cast<uint4*>(row + (c >> 1) * SPAN + (((4 * (c & 1) + u) ^ (i & 7)) << 4)) = numbers(code[u], s2, m2);
             }
-            page = page1;
-            grp = grp1;
+            fence_proxy_async_smem();
+            mbar_arrive(full + s);
+            load(j + 1, next);                                            // a tile ahead (behind the fence, which would wait for it)
+            next = page_of(j + 2);
         }
     } else {
         // ------------------------------------------------------------------ softmax rows
@@ -410,7 +409,7 @@ kv4_prefill_kernel(const Args a) {
         tcgen05_fence_before();
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -444,7 +443,12 @@ VOB_EXPORT int vob_kv4_prefill(const void* q, long long q_stride, void* out, lon
     if (hd > 128 || group > BM || S > 65535) return VOB_ERR_UNSUPPORTED;
     const long long tokens = 2 * (BM / group), row_tiles = ((long long)max_new + tokens - 1) / tokens;
     if (row_tiles > 65535) return VOB_ERR_UNSUPPORTED;
+    const unsigned p8 = (unsigned)page_size / 8;
+    const unsigned magic = p8 == 1 ? 0u : (unsigned)(((1ull << 32) + p8 - 1) / p8);
+    // exact while (key / 8) * (magic * p8 - 2^32) < 2^32: always for powers of two, else for key * page_size up to 2^38
+    const unsigned long long over = p8 == 1 ? 0 : (unsigned long long)magic * p8 - (1ull << 32);
+    if ((unsigned long long)max_pages * p8 * over >= (1ull << 32) || (long long)max_pages * page_size > 0x7fffff00LL) return VOB_ERR_UNSUPPORTED;
     const Args a = {(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, (const unsigned char*)cache, tables, seq_starts, context_lens, err,
-                    max_pages, (int)num_pages, H, G, hd, page_size, window, scale * 1.4426950408889634f};
+                    max_pages, (int)num_pages, H, G, hd, page_size, window, scale * 1.4426950408889634f, magic};
     return hd <= 64 ? launch<64>(a, S, row_tiles, stream) : launch<128>(a, S, row_tiles, stream);
 }
