@@ -10,10 +10,11 @@
 //     pages, 128 contiguous bytes per eight keys), and writes K and V as bfloat16 into the swizzled operand tiles: per 8 codes 3 shifts,
 //     4 and-ors (a code in the low mantissa bits of 128 is 128 + n), 4 subtractions, 4 FMAs and one 16-byte store. The pairs that this gives are numbers
 //     (0,4), (1,5), (2,6), (3,7) of every eight; they stay in that order in the tiles, q is laid out likewise and the sums are put back at the end;
-//   * one thread issues S = Q K^T and O += P V (tcgen05.mma; S, P and O in tensor memory: S0 128 | S1 128 | O0 | O1 columns, P over its S);
-//   * two times four warps, a row a thread, do the softmax of the two row tiles: while one tile's rows work the tensor cores
-//     work for the other. P goes back in two halves, the first product starting on the first.
-// The running maximum moves only where a tile's exceeds it by more than 2^8 (sums, P and O share the reference), so O is rescaled rarely.
+//   * a thread for each row tile issues its S = Q K^T and O += P V in steps of 64 keys (tcgen05.mma; S, P and O in tensor memory: two S of 64 columns per row
+//     tile, P over its S, O0, O1). The scores of step u + 2 are asked for once P V of step u is done, while the rows
+//     work on step u + 1;
+//   * two times four warps, a row a thread, do the softmax of the two row tiles.
+// The maximum that P is relative to moves only where a row's sum over a step passes 2^10, so most steps take no maximum and O is rescaled rarely.
 // A key that is not finite is seen as NaN by the rows that see it, and by no other; its value is 0 in the tile.
 //
 // Every wait is bounded (sm100.cuh); on expiry the block raises the error flag, frees its tensor memory and returns.
@@ -25,14 +26,15 @@ namespace {
 using namespace vob_kv4;
 using namespace vob_sm100;
 
-constexpr int BM = 128, BN = 128;                     // rows of a row tile, keys of a key tile
-// Five warpgroups: softmax of the row tiles (2), codes to numbers of K and of V, issue of products (one thread). The registers that a block of 640
+constexpr int BM = 128, BN = 128, BS = 64;            // rows of a row tile, keys of a key tile, keys of a softmax step
+// Five warpgroups: softmax of the row tiles (2), codes to numbers of K and of V, issue of products (two threads). The registers that a block of 640
 // threads is launched with, 96 each, are shared out anew.
 constexpr int NTHREADS = 640;
 constexpr int REGS_ROWS = 136, REGS_CODES = 72, REGS_ISSUE = 64;
 static_assert(2 * REGS_ROWS + 2 * REGS_CODES + REGS_ISSUE == 5 * 96, "no more than the launch's registers");
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr float FLT_LOWEST = -3.4028234663852886e38f;
 constexpr int SPAN = 128 * 128;                       // bytes of 128 rows of 64 bfloat16
 
 struct Args {
@@ -62,9 +64,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The larger, NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -109,17 +112,17 @@ kv4_prefill_kernel(const Args a) {
     uint64_t* q_ready = bars;                // [2] a row tile's Q is in shared memory
     uint64_t* k_full = bars + 2;             // [2] 128 threads have written the stage
     uint64_t* v_full = bars + 4;             // [2]
-    uint64_t* k_free = bars + 6;             // [2] the products that read the stage are done
+    uint64_t* k_free = bars + 6;             // [2] the products of both row tiles that read the stage are done
     uint64_t* v_free = bars + 8;             // [2]
-    uint64_t* s_full = bars + 10;            // [2] a row tile's scores are there
-    uint64_t* p_first = bars + 12;           // [2] its 128 rows have written P of the tile's first 64 keys
-    uint64_t* p_second = bars + 14;          // [2] and of the others
-    uint64_t* o_full = bars + 16;            // [2] its O holds the tile
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
+    uint64_t* s_full = bars + 10;            // [2 row tiles][2 buffers] scores of 64 keys are there
+    uint64_t* p_ready = bars + 14;           // [2][2] the tile's 128 rows have written P over them
+    uint64_t* o_full = bars + 18;            // [2] a row tile's O holds a step
+    uint64_t* o_done = bars + 20;            // [2] and all of them (a barrier of its own: who waits for a phase must know that the one before it has passed)
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // key tiles [from[t], to[t]) of each row tile
+    // steps of 64 keys [from[t], to[t]) of each row tile, beginning with a key tile
     int from[2], to[2], hi = 0, lo = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -127,25 +130,28 @@ kv4_prefill_kernel(const Args a) {
         from[t] = to[t] = 0;
         if (r0 < r1) {
             const int h = ctx + (r1 - 1) / group + 1, l = a.window ? max(0, ctx + r0 / group - a.window + 1) : 0;
-            from[t] = l / BN;
-            to[t] = (h + BN - 1) / BN;
+            from[t] = l / BN * 2;
+            to[t] = (h + BS - 1) / BS;
             hi = max(hi, h);
             lo = min(lo, l);
         }
     }
-    const int j0 = from[0], j1 = max(to[0], to[1]);                    // the first tile has rows, and sees the earliest keys
+    const int u0 = from[0], u1 = max(to[0], to[1]);                    // the first row tile has rows, and sees the earliest keys
+    const int j0 = u0 / 2, j1 = (u1 + 1) / 2;                          // key tiles
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_ready + i, 128);
             mbar_init(k_full + i, 128);
             mbar_init(v_full + i, 128);
-            mbar_init(k_free + i, 1);
-            mbar_init(v_free + i, 1);
+            mbar_init(k_free + i, 2);
+            mbar_init(v_free + i, 2);
             mbar_init(s_full + i, 1);
-            mbar_init(p_first + i, 128);
-            mbar_init(p_second + i, 128);
+            mbar_init(s_full + 2 + i, 1);
+            mbar_init(p_ready + i, 128);
+            mbar_init(p_ready + 2 + i, 128);
             mbar_init(o_full + i, 1);
+            mbar_init(o_done + i, 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -163,56 +169,63 @@ kv4_prefill_kernel(const Args a) {
     if (warp >= 16) {
         // ------------------------------------------------------------------ products
         regs_down<REGS_ISSUE>();
-        if (warp == 16 && elect_one()) {
-            constexpr uint32_t idesc_qk = umma_idesc_bf16(BM, BN, false), idesc_pv = umma_idesc_bf16(BM, HD, true);
+        const int t = warp - 16;                                          // a thread issues the products of one row tile
+        if (t < 2 && elect_one()) {
+            constexpr uint32_t idesc_qk = umma_idesc_bf16(BM, BS, false), idesc_pv = umma_idesc_bf16(BM, HD, true);
+            const int t_from = t ? from[1] : from[0], t_to = t ? to[1] : to[0];
+            const uint32_t tS = tmem + t * BN, tO = tmem + 2 * BN + t * HD;
             bool ok = true;
-            auto issue_qk = [&](int t, int j) {
+            // a key tile that the row tile does not look at
+            auto skip = [&](int j) {
                 const int s = (j - j0) & 1;
-                ok = ok && mbar_wait(q_ready + t, 0, abort_flag, a.err, 41) && mbar_wait(k_full + s, ((j - j0) >> 1) & 1, abort_flag, a.err, 42);
+                const uint32_t ph = ((j - j0) >> 1) & 1;
+                ok = ok && mbar_wait(k_full + s, ph, abort_flag, a.err, 41) && mbar_wait(v_full + s, ph, abort_flag, a.err, 41);
+                if (!ok) return;
+                mbar_arrive(k_free + s);
+                mbar_arrive(v_free + s);
+            };
+            auto issue_qk = [&](int u) {
+                const int m = (u >> 1) - j0, s = m & 1, b = u & 1;
+                if (!b) ok = ok && mbar_wait(k_full + s, (m >> 1) & 1, abort_flag, a.err, 42);
                 if (!ok) return;
                 tcgen05_fence_after();
 #pragma unroll
                 for (int h = 0; h < NS; ++h) {
-                    const uint64_t qd = umma_desc_sw128(sQ + t * TILE + h * SPAN), kd = umma_desc_sw128(sK + s * TILE + h * SPAN);
+                    const uint64_t qd = umma_desc_sw128(sQ + t * TILE + h * SPAN), kd = umma_desc_sw128(sK + s * TILE + h * SPAN + b * (BS * 128));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_bf16(tmem + t * BN, qd + 2 * k, kd + 2 * k, idesc_qk, (h > 0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) umma_bf16(tS + b * BS, qd + 2 * k, kd + 2 * k, idesc_qk, (h > 0 || k > 0) ? 1u : 0u);
                 }
-                umma_commit(s_full + t);
+                umma_commit(s_full + 2 * t + b);
+                if (b || u + 1 == t_to) umma_commit(k_free + s);
             };
-#pragma unroll 1
-            for (int t = 0; t < 2; ++t)
-                if ((t ? from[1] : from[0]) == j0 && (t ? to[1] : to[0]) > j0) issue_qk(t, j0);
-            if (ok) umma_commit(k_free);
-            for (int j = j0; j < j1 && ok; ++j) {
-                const int s = (j - j0) & 1;
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
-                    const int t_from = t ? from[1] : from[0], t_to = t ? to[1] : to[0];
-                    if (j >= t_from && j < t_to) {
-                        const int n = j - t_from;
-                        const uint64_t vd = umma_desc_sw128(sV + s * TILE, SPAN);
-                        const uint32_t tO = tmem + 2 * BN + t * HD, tP = tmem + t * BN;
-                        ok = ok && mbar_wait(v_full + s, ((j - j0) >> 1) & 1, abort_flag, a.err, 43) &&
-                             mbar_wait(p_first + t, n & 1, abort_flag, a.err, 44);
-                        if (!ok) break;
-                        tcgen05_fence_after();
+            const int j_from = t_from < t_to ? t_from / 2 : j1, j_to = t_from < t_to ? (t_to + 1) / 2 : j1;
+            for (int j = j0; j < j_from && ok; ++j) skip(j);
+            if (t_from < t_to) {
+                ok = ok && mbar_wait(q_ready + t, 0, abort_flag, a.err, 43);
+                issue_qk(t_from);
+                if (t_from + 1 < t_to) issue_qk(t_from + 1);
+            }
+            for (int u = t_from; u < t_to && ok; ++u) {
+                const int m = (u >> 1) - j0, s = m & 1, b = u & 1, n = u - t_from;
+                if (!b) ok = mbar_wait(v_full + s, (m >> 1) & 1, abort_flag, a.err, 44);
+                ok = ok && mbar_wait(p_ready + 2 * t + b, (n >> 1) & 1, abort_flag, a.err, 45);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint64_t vd = umma_desc_sw128(sV + s * TILE + b * (BS * 128), SPAN);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_bf16_ts(tO, tP + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, (n > 0 || k > 0) ? 1u : 0u);
-                        ok = mbar_wait(p_second + t, n & 1, abort_flag, a.err, 45);
-                        if (!ok) break;
-                        tcgen05_fence_after();
-#pragma unroll
-                        for (int k = 4; k < 8; ++k) umma_bf16_ts(tO, tP + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, 1u);
-                        umma_commit(o_full + t);
-                    }
-                    if (j + 1 >= t_from && j + 1 < t_to) issue_qk(t, j + 1);
-                }
-                if (ok) {
-                    umma_commit(v_free + s);
-                    umma_commit(k_free + (s ^ 1));
+                for (int k = 0; k < 4; ++k)                               // 16 keys: 8 columns of P, 16 rows of V
+                    umma_bf16_ts(tO, tS + b * BS + 8 * k, vd + (uint64_t)k * (2048 >> 4), idesc_pv, (n > 0 || k > 0) ? 1u : 0u);
+                umma_commit(o_full + t);
+                if (u + 1 == t_to) umma_commit(o_done + t);
+                if (b || u + 1 == t_to) umma_commit(v_free + s);
+                if (u + 2 < t_to) {
+                    // the scores of step u + 2 lie over this step's P, whose product must be done: products with different accumulators are not
+                    // ordered by being issued one behind the other. (The other row tile's keep the tensor cores busy meanwhile.)
+                    ok = mbar_wait(o_full + t, n & 1, abort_flag, a.err, 47);
+                    if (ok) issue_qk(u + 2);
                 }
             }
+            for (int j = j_to; j < j1 && ok; ++j) skip(j);
         }
         __syncwarp();
     } else if (warp >= 8) {
@@ -303,68 +316,39 @@ kv4_prefill_kernel(const Args a) {
             mbar_arrive(q_ready + t);
         }
         const uint32_t lane_at = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t tS = lane_at + t * BN, tO = lane_at + 2 * BN + t * HD;
+        const uint32_t tO = lane_at + 2 * BN + t * HD;
         float m_ref = -INFINITY, l = 0.f;
+        bool nan_row = false;                                            // the row sees a key that is NaN
         bool ok = true;
         auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // tcgen05.ld / st are warp-wide: a warp gives up as a whole
             return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.err, code) ? 1 : 0) != 0;
         };
-        for (int j = t_from; j < t_to && ok; ++j) {
-            const int n = j - t_from, kbase = j * BN;
-            const bool masked = kbase + BN - 1 > first_pos || (a.window && kbase <= last_pos - a.window);
-            const int see_from = a.window ? pos - a.window + 1 - kbase : -0x7fffffff, see_to = pos - kbase;      // keys of the tile that the row sees
-            if (!wait_all(s_full + t, n & 1, 48)) { ok = false; break; }
+        for (int u = t_from; u < t_to && ok; ++u) {
+            const int n = u - t_from, kbase = u * BS, b = u & 1;
+            const uint32_t tS = lane_at + t * BN + b * BS;
+            const bool masked = kbase + BS - 1 > first_pos || (a.window && kbase <= last_pos - a.window);
+            if (!wait_all(s_full + 2 * t + b, (n >> 1) & 1, 48)) { ok = false; break; }
             tcgen05_fence_after();
             uint32_t va[32], vb[32];
-            auto scores = [&](int half) {
-                tmem_ld32(tS + 64 * half, va);
-                tmem_ld32(tS + 64 * half + 32, vb);
-                tmem_wait_ld();
-                if (masked) {
+            tmem_ld32(tS, va);
+            tmem_ld32(tS + 32, vb);
+            tmem_wait_ld();
+            if (masked) {
+                const int see_from = a.window ? pos - a.window + 1 - kbase : -0x7fffffff, see_to = pos - kbase;      // keys of the step that the row sees
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int k = 64 * half + i;
-                        if (k > see_to || k < see_from) va[i] = 0xff800000u;             // -inf
-                        if (k + 32 > see_to || k + 32 < see_from) vb[i] = 0xff800000u;
-                    }
-                }
-            };
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-            for (int half = 1; half >= 0; --half) {
-                scores(half);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    mx0 = max3(mx0, __uint_as_float(va[i]), __uint_as_float(vb[i]));
-                    mx1 = max3(mx1, __uint_as_float(va[i + 1]), __uint_as_float(vb[i + 1]));
+                for (int i = 0; i < 32; ++i) {
+                    if (i > see_to || i < see_from) va[i] = 0xff800000u;                     // -inf
+                    if (i + 32 > see_to || i + 32 < see_from) vb[i] = 0xff800000u;
                 }
             }
-            const float mx2 = fmaxf(mx0, mx1) * a.scale_log2;            // scale > 0: the maximum commutes
-            const bool grow = mx2 > m_ref + 8.f;                         // also the first finite maximum
-            const float m_new = grow ? mx2 : m_ref;
-            const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.f;   // m_ref = -inf: 0
-            m_ref = m_new;
-            l *= alpha;
-            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-            if (n > 0 && __any_sync(0xffffffffu, grow)) {
-                if (!wait_all(o_full + t, (n - 1) & 1, 49)) { ok = false; break; }
-                tcgen05_fence_after();
-#pragma unroll
-                for (int c = 0; c < HD; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(tO + c, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-                    tmem_st16(tO + c, v);
-                }
-            }
-            const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-m_use, -m_use);
-            float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (half) scores(1);
-                auto weigh = [&](const uint32_t (&v)[32], float2& acc, uint32_t to_column) {
+            // P = 2^(score - m_ref) over the scores, and their sum. m_ref is some maximum of earlier steps: as long as no row's sum passes 2^10 it
+            // may stay, since P, the sums and O are floating-point numbers relative to it.
+            const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
+            float sum;
+            auto weigh = [&]() {
+                const float2 nm2 = make_float2(-m_ref, -m_ref);
+                float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+                auto half = [&](const uint32_t (&v)[32], float2& acc, uint32_t to_column) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
@@ -373,19 +357,54 @@ kv4_prefill_kernel(const Args a) {
                         acc = __fadd2_rn(acc, p);
                         pk[i >> 1] = pack_bf16(p.x, p.y);
                     }
-                    tmem_st16(tS + to_column, pk);                        // over scores that are in registers or done with
+                    tmem_st16(tS + to_column, pk);                        // over scores that are in registers
                 };
-                weigh(va, acc0, 32 * half);
-                weigh(vb, acc1, 32 * half + 16);
-                tmem_wait_st();
-                tcgen05_fence_before();
-                mbar_arrive((half ? p_second : p_first) + t);
+                half(va, acc0, 0);
+                half(vb, acc1, 16);
+                sum = (acc0.x + acc0.y) + (acc1.x + acc1.y);
+            };
+            bool move = n == 0;
+            if (!move) {
+                weigh();
+                move = __any_sync(0xffffffffu, !(sum <= 1024.f));
             }
-            l += (acc0.x + acc0.y) + (acc1.x + acc1.y);
+            if (move) {
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    mx0 = max3(mx0, __uint_as_float(va[i]), __uint_as_float(vb[i]));
+                    mx1 = max3(mx1, __uint_as_float(va[i + 1]), __uint_as_float(vb[i + 1]));
+                }
+                mx0 = max3(mx0, mx1, mx1);
+                nan_row = nan_row || mx0 != mx0;
+                const float m_new = fmaxf(m_ref, mx0 * a.scale_log2);    // scale > 0: the maximum commutes. NaN: m_ref stays
+                const float alpha = m_ref < m_new ? exp2_fast(m_ref - m_new) : 1.f;       // m_ref = -inf: 0
+                m_ref = m_new == -INFINITY ? FLT_LOWEST : m_new;         // a row that has seen nothing: 2^(-inf + that) = 0
+                l *= alpha;
+                if (n > 0) {
+                    // O may be touched once the product of the step before is done
+                    if (!wait_all(o_full + t, (n - 1) & 1, 49)) { ok = false; break; }
+                    tcgen05_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(tO + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st16(tO + c, v);
+                    }
+                }
+                weigh();
+            }
+            tmem_wait_st();
+            tcgen05_fence_before();
+            mbar_arrive(p_ready + 2 * t + b);
+            l += sum;
         }
-        if (ok && t_to > t_from && wait_all(o_full + t, (t_to - t_from - 1) & 1, 50)) {
+        if (ok && t_to > t_from && wait_all(o_done + t, 0, 50)) {
             tcgen05_fence_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = nan_row ? NAN : l == 0.f ? 0.f : 1.f / l;
             __nv_bfloat16* dst = a.out + at * a.out_stride + (size_t)head * a.hd;
 #pragma unroll
             for (int c = 0; c < HD; c += 16) {
