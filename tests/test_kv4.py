@@ -39,7 +39,7 @@ def test_there_is_no_cpu_path():
 @pytest.fixture
 def no_gpu(monkeypatch):
     """The wrappers' checks on CPU tensors: the device's check passes, a launch is a failure."""
-    monkeypatch.setattr(kernels, "_cuda", lambda *a: None)
+    monkeypatch.setattr(kernels, "_kv4_device", lambda *a: 0)
 
     def launch(*a):
         raise AssertionError("a launch was reached")

@@ -33,21 +33,22 @@ using namespace vob_kv4;
 using vob_sm100::smem_u32;
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int TILE = 32;                   // keys of a warp's step
-constexpr int ROUND = TILE * WARPS;        // keys of a block's step
+constexpr int STEP = 32;                   // keys of a warp's step
 constexpr float P_LIMIT = 32768.f, P_TOP = 4.f;
 
 // NC chunks of 32 numbers, NT times 8 heads. Blocks per SM and stages of a warp's ring: as many bytes in flight as registers and
 // shared memory allow (4 blocks of 4 warps at head sizes up to 128).
 template <int NC, int NT> struct Sizes {
     static constexpr int SUB = 256 * NC + 64;                     // bytes of eight keys and values
+    static constexpr int TILE = NC <= 2 ? 64 : 32;                // keys of a stage of a warp's ring: one or two steps
+    static constexpr int ROUND = TILE * WARPS;                    // keys that a block takes at a time
     static constexpr int STAGE = SUB * (TILE / GROUP);
     static constexpr int BLOCKS = NC > 4 || NC * NT > 4 ? 2 : NC * NT == 4 ? 3 : 4 - (NT - 1);
-    static constexpr int STAGES = NC <= 2 ? 5 : NC > 4 ? 3 : NT == 2 ? 5 : NC == 4 ? 4 : 3;
+    static constexpr int STAGES = NC > 4 || NC <= 2 ? 3 : NT == 2 ? 5 : NC == 4 ? 4 : 3;
     static constexpr int HEADS = 8 * NT;
     static constexpr int OSTRIDE = 32 * NC + 8;                   // a head's sums in a stage, padded: 8 heads fill it exactly
     static constexpr int PARTIAL = HEADS * (32 * NC + 2);         // floats of a partial result
-    static_assert(8 * OSTRIDE * 4 == STAGE, "the warps' sums of 8 heads use a stage of the ring");
+    static_assert(8 * OSTRIDE * 4 <= STAGE, "the warps' sums of 8 heads use a stage of the ring");
 };
 
 struct Args {
@@ -95,9 +96,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // A request's keys lo .. hi - 1, in rounds t0 .. t0 + count - 1. (A position behind the request's block table counts as one key behind it, which makes
 // the row NaN.)
-struct Span {
+template <int ROUND> struct SpanOf {
     int lo, hi, t0, count;
-    __device__ __forceinline__ Span(int pos, int window, int table_keys) {
+    __device__ __forceinline__ SpanOf(int pos, int window, int table_keys) {
         hi = min(max(pos, -1), table_keys) + 1;
         lo = window ? max(0, hi - window) : 0;
         t0 = lo / ROUND;
@@ -114,6 +115,8 @@ template <int NC, int NT>
 __global__ void __launch_bounds__(THREADS, Sizes<NC, NT>::BLOCKS)
 kv4_decode_kernel(const Args a) {
     using Z = Sizes<NC, NT>;
+    using Span = SpanOf<Z::ROUND>;
+    constexpr int TILE = Z::TILE, ROUND = Z::ROUND;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem;                                                    // [WARPS][STAGES][STAGE]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * Z::STAGES * Z::STAGE);    // [WARPS][STAGES]
@@ -184,8 +187,11 @@ kv4_decode_kernel(const Args a) {
     Place ld = at;                                                                 // the next round to fetch from
     int ld_x = x0;
     Span ld_span(a.positions[ld.s], a.window, a.table_keys);
-    int batch_k = -1, batch_end = -1;                                              // rounds of the unit whose pages the lanes hold
-    int page = 0, page_off = 0;                                                    // of piece lane % pieces of round batch_k + lane / pieces
+    // A lane holds where piece lane % pieces of round batch_k + lane / pieces comes from; which lanes' pieces there are, and which of them lie in
+    // pages outside the pool.
+    int batch_k = 0, batch_end = -1;
+    const unsigned char* src = nullptr;
+    unsigned there = 0, wrong = 0;
     int stage_in = 0, issued = 0, taken = 0;
     bool dead = false;                                                              // a wait ran out: nothing more is fetched or waited for
     auto fetch = [&]() {
@@ -193,40 +199,42 @@ kv4_decode_kernel(const Args a) {
             const int base = (ld_span.t0 + ld.k) * ROUND + warp * TILE;
             const bool any = base < ld_span.hi && base + TILE > ld_span.lo;
             if (any) {
-                const int per_batch = 32 / pieces;
-                if (batch_k < 0 || ld.k >= batch_end) {
+                if (ld.k >= batch_end) {
                     batch_k = ld.k;
-                    batch_end = batch_k + per_batch;
+                    batch_end = batch_k + 32 / pieces;
                     const int key = (ld_span.t0 + batch_k + lane / pieces) * ROUND + warp * TILE + (lane % pieces) * piece;
                     const int idx = key / a.page_size;
-                    page_off = key - idx * a.page_size;
-                    page = -2;                                                      // nothing to fetch
-                    if (key < ld_span.hi && key + piece > ld_span.lo) page = idx < a.max_pages ? a.tables[(size_t)ld.s * a.max_pages + idx] : -1;
+                    const bool want = key < ld_span.hi && key + piece > ld_span.lo;
+                    int page = -1;
+                    if (want && idx < a.max_pages) page = a.tables[(size_t)ld.s * a.max_pages + idx];
+                    const bool good = page >= 0 && page < a.num_pages;
+                    there = __ballot_sync(0xffffffffu, good);
+                    wrong = __ballot_sync(0xffffffffu, want && !good);
+                    src = a.cache + (((size_t)(good ? page : 0) * a.G + ld.gh / a.head_tiles) * a.page_size + (key - idx * a.page_size)) * width;
                 }
-                const bool mine = lane / pieces == ld.k - batch_k;
-                const bool want = mine && page != -2, good = want && page >= 0 && page < a.num_pages;
-                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * piece_bytes;
-                const uint32_t bar = bar_at + 8 * stage_in, dst = ring_at + stage_in * Z::STAGE + (lane % pieces) * piece_bytes;
-                if (__any_sync(0xffffffffu, want && !good)) {
+                const int shift = (ld.k - batch_k) * pieces;
+                const unsigned mine = (1u << pieces) - 1u;
+                const uint32_t dst = ring_at + stage_in * Z::STAGE + (lane - shift) * piece_bytes;
+                const bool here = (unsigned)(lane - shift) < (unsigned)pieces;
+                if (wrong >> shift & mine) {
                     // a page outside the pool: NaN where its scales would be
-                    if (want && !good)
+                    if (here && (wrong >> lane & 1))
                         for (int i = 0; i < piece; ++i)
-                            *reinterpret_cast<uint2*>(my_ring + stage_in * Z::STAGE + (lane % pieces) * piece_bytes + (i >> 3) * Z::SUB + 256 * NC + 8 * (i & 7)) =
+                            *reinterpret_cast<uint2*>(my_ring + stage_in * Z::STAGE + (lane - shift) * piece_bytes + (i >> 3) * Z::SUB + 256 * NC + 8 * (i & 7)) =
                                 make_uint2(0x7fff7fffu, 0x7fff7fffu);
                     vob_sm100::fence_proxy_async_smem();
                     __syncwarp();
                 }
-                if (lane == 0) vob_sm100::mbar_expect_tx(bars + warp * Z::STAGES + stage_in, bytes);
+                if (lane == 0) vob_sm100::mbar_expect_tx(bars + warp * Z::STAGES + stage_in, __popc(there >> shift & mine) * piece_bytes);
                 __syncwarp();
-                if (good)
-                    bulk_load(dst, a.cache + (((size_t)page * a.G + ld.gh / a.head_tiles) * a.page_size + page_off) * width, piece_bytes, bar);
+                if (here && (there >> lane & 1)) bulk_load(dst, src, piece_bytes, bar_at + 8 * stage_in);
                 stage_in = stage_in + 1 == Z::STAGES ? 0 : stage_in + 1;
                 ++issued;
             }
             ++ld_x;
             if (++ld.k == ld_span.count) {
                 ld.k = 0;
-                batch_k = -1;
+                batch_end = -1;
                 if (++ld.gh == GH) {
                     ld.gh = 0;
                     while (ld_x < x1) {
@@ -334,10 +342,15 @@ kv4_decode_kernel(const Args a) {
             }
             ++taken;
             my_stage = stage_out;
-            const unsigned char* st = my_ring + stage_out * Z::STAGE;
-            const uint32_t st_at = ring_at + stage_out * Z::STAGE;
+            const int stage = stage_out;
             if (++stage_out == Z::STAGES) { stage_out = 0; phase ^= 1; }
             worked = true;
+#pragma unroll 1
+            for (int sub = 0; sub < TILE / STEP; ++sub) {
+            const int first_key = base + sub * STEP;
+            if (TILE > STEP && !(first_key < span.hi && first_key + STEP > span.lo)) continue;
+            const unsigned char* st = my_ring + stage * Z::STAGE + sub * (STEP / GROUP) * Z::SUB;
+            const uint32_t st_at = ring_at + stage * Z::STAGE + sub * (STEP / GROUP) * Z::SUB;
 
             // scores of 32 keys: two tiles of 16
             float s[2][NT][4];
@@ -368,7 +381,8 @@ kv4_decode_kernel(const Args a) {
             // scales and minima of this lane's keys g8, g8 + 8, + 16, + 24
             float2 ks[4], vs[4];
             float vt[4];                                                             // the value's scale, as the reference takes it
-            bool seen[4] = {true, true, true, true};
+            const bool edge = first_key < span.lo || first_key + STEP > span.hi;
+            unsigned seen = 15u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint2 w = *reinterpret_cast<const uint2*>(st + i * Z::SUB + 256 * NC + 8 * g8);
@@ -376,37 +390,45 @@ kv4_decode_kernel(const Args a) {
                 vs[i] = scale_min(w.y);
                 ks[i].x *= to_score;
             }
-            const bool edge = base < span.lo || base + TILE > span.hi;
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int j = base + 8 * i + g8;
-                    seen[i] = j >= span.lo && j < span.hi;
-                    if (!seen[i]) { ks[i] = make_float2(0.f, 0.f); vs[i] = make_float2(0.f, 0.f); }   // whatever lies there
+                    const int j = first_key + 8 * i + g8;
+                    if (j < span.lo || j >= span.hi) {                               // whatever lies there
+                        seen &= ~(1u << i);
+                        ks[i] = vs[i] = make_float2(0.f, 0.f);
+                    }
                 }
             }
             // below 2^-40 a scale counts as that: p itself stays below 2^55, whatever the values of the keys with large scores
 #pragma unroll
             for (int i = 0; i < 4; ++i) vt[i] = vs[i].x < 9.094947e-13f ? 9.094947e-13f : vs[i].x;
-            float p[2][NT][4];
-            bool over = false;
+            float p[2][NT][4], most = 0.f;                                           // the largest p_j times scale
             auto weigh = [&](int n) {
-                bool past = false;
+                float e[4][2];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int key = 0; key < 4; ++key)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = 2 * t + (i >> 1);
-                        float e = exp2_fast(fmaf(s[t][n][i], ks[key].x, fmaf(ks[key].y, qs[n][i & 1], -ref[n][i & 1])));
-                        if (edge && !seen[key]) e = 0.f;
-                        p[t][n][i] = e;
-                        past = past || !(e * vt[key] <= P_LIMIT);
+                    for (int h = 0; h < 2; ++h) e[key][h] = fmaf(ks[key].y, qs[n][h], -ref[n][h]);
+                if (edge) {
+#pragma unroll
+                    for (int key = 0; key < 4; ++key)
+                        if (!(seen >> key & 1)) e[key][0] = e[key][1] = -INFINITY;
+                }
+#pragma unroll
+                for (int key = 0; key < 4; ++key) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float x = exp2_fast(fmaf(s[key >> 1][n][2 * (key & 1) + h], ks[key].x, e[key][h]));
+                        p[key >> 1][n][2 * (key & 1) + h] = x;
+                        e[key][h] = x;
                     }
-                return past;
+                    most = fmaxf(most, fmaxf(e[key][0], e[key][1]) * vt[key]);       // (NaN is left out: it stays in p)
+                }
             };
 #pragma unroll
-            for (int n = 0; n < NT; ++n) over = weigh(n) || over;
-            if (__any_sync(0xffffffffu, over)) {
+            for (int n = 0; n < NT; ++n) weigh(n);
+            if (__any_sync(0xffffffffu, most > P_LIMIT)) {
                 // a new reference: the largest score + log2 of its value's scale
                 float lg[4];
 #pragma unroll
@@ -420,7 +442,7 @@ kv4_decode_kernel(const Args a) {
                         for (int i = 0; i < 4; ++i) {
                             const int key = 2 * t + (i >> 1);
                             const float y = fmaf(s[t][n][i], ks[key].x, ks[key].y * qs[n][i & 1]) + lg[key];
-                            if (seen[key]) top[i & 1] = fmaxf(top[i & 1], y);
+                            if (seen >> key & 1) top[i & 1] = fmaxf(top[i & 1], y);
                         }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -468,6 +490,7 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) w[i] >>= 8;
                 }
+            }
             }
             __syncwarp();                                                            // every lane has read the stage: it may be fetched into
         }
@@ -647,7 +670,7 @@ VOB_EXPORT int vob_kv4_decode(const void* q, long long q_stride, void* out, long
     a.head_tiles = (H / G + heads - 1) / heads;
     if (counters < (long long)S * G * a.head_tiles) return VOB_ERR_BAD_ARG;
     const long long keys = window ? min((long long)max_pages * page_size, (long long)window) : (long long)max_pages * page_size;
-    const long long rounds = keys / ROUND + 2;
+    const long long rounds = keys / (STEP * WARPS) + 2;                              // of the shortest that a size has
     if ((long long)max_pages * page_size > 0x7ffffff0LL || rounds * S * G * a.head_tiles > 0x7fffffffLL) return VOB_ERR_UNSUPPORTED;
     a.table_keys = max_pages * page_size;
     switch (chunks(hd) * 2 + (heads == 16)) {

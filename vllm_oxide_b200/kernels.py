@@ -2248,26 +2248,52 @@ def kv4_supported(num_heads: int, num_kv_heads: int, head_dim: int, page_size: i
             and page_size > 0 and page_size % 8 == 0)
 
 
+# The wrappers below are called once or more per layer of a decode step whose kernels take some microseconds: their checks read each of a
+# tensor's properties once, and pointers go to ctypes as plain integers.
+def _kv4_device(op, *tensors) -> int:
+    """The current device, on which all of the tensors must be (launches go to its current stream)."""
+    first = tensors[0].get_device()
+    dev = torch._C._cuda_getDevice() if first >= 0 else -1
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or first < 0):
+            _cuda(op, *tensors)
+            raise ShapeError(op, f"the tensors are on {t.device}, the current device is cuda:{dev}: launches go to its stream")
+    return dev
+
+
 def _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim):
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != num_kv_heads or cache.shape[3] != kv4_width(head_dim) \
-            or not cache.is_contiguous() or cache.shape[0] < 1:
+    """(pages, page size) of a cache that fits."""
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != 32 * -(-head_dim // 32) + 8 \
+            or not cache.is_contiguous() or shape[0] < 1:
         raise ShapeError(op, f"the cache must be contiguous uint8 [pages, {num_kv_heads}, page_size, {kv4_width(head_dim)}], got "
-                             f"{cache.dtype} {list(cache.shape)}")
-    if cache.shape[0] * cache.shape[2] > 2 ** 31 - 1:
-        raise ShapeError(op, f"{cache.shape[0]} pages of {cache.shape[2]} tokens are beyond 2^31 - 1 slots")
+                             f"{cache.dtype} {list(shape)}")
+    pages, page = shape[0], shape[2]
+    if pages * page > 2 ** 31 - 1:
+        raise ShapeError(op, f"{pages} pages of {page} tokens are beyond 2^31 - 1 slots")
     if cache.data_ptr() % 16:
         raise ShapeError(op, "the cache must start on a 16-byte boundary")
-    if cache.is_cuda and cache.device.index != torch.cuda.current_device():
-        raise ShapeError(op, f"the tensors are on {cache.device}, the current device is cuda:{torch.cuda.current_device()}: launches go to its stream")
-    if not kv4_supported(num_heads, num_kv_heads, head_dim, cache.shape[2]):
+    if not kv4_supported(num_heads, num_kv_heads, head_dim, page):
         raise ShapeError(op, f"sizes not supported: heads {num_heads}/{num_kv_heads}, head_dim {head_dim} (multiples of 16 up to 256), "
-                             f"page {cache.shape[2]} (multiples of 8)")
+                             f"page {page} (multiples of 8)")
+    return pages, page
 
 
-def _kv4_rows(op, name, t, rows, cols, dtype):
-    _rows_2d(t, op, name)
-    if t.shape != (rows, cols) or t.dtype != dtype:
-        raise ShapeError(op, f"{name} must be {dtype} [{rows}, {cols}], got {t.dtype} {list(t.shape)}")
+def _kv4_rows(op, name, t, rows, cols, dtype) -> int:
+    """The row stride of a [rows, cols] tensor of this type with unit inner stride (`rows` None: any number)."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or shape[1] != cols or t.dtype is not dtype or strides[1] != 1:
+        raise ShapeError(op, f"{name} must be {dtype} [{'T' if rows is None else rows}, {cols}] with unit inner stride, got {t.dtype} {list(shape)} "
+                             f"strides {list(strides)}")
+    return strides[0]
+
+
+_KV4_APPEND = [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P]
+_KV4_READ = [_P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P]
+_KV4_ATTEND = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P]
+_KV4_DECODE = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P, _L, _I, _P, _P]
+_KV4_PREFILL = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P]
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 @_timed
@@ -2279,25 +2305,27 @@ def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     wider tensor; k and v are left as they are. A token whose slot is negative (or `slots` None, or a slot behind the pool) is not
     kept; no two tokens of one call may have the same slot. A key or value with a number that is not finite is kept as NaN."""
     op = "kv4_append"
-    _cuda(op, q, k, v, positions, slots, inv_freq, cache, q_out)
-    _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
-    _rows_2d(q, op, "q")
-    T, code = q.shape[0], _code(q, op)
-    _kv4_rows(op, "q", q, T, num_heads * head_dim, q.dtype)
-    for name, t in (("k", k), ("v", v)):
-        _kv4_rows(op, name, t, T, num_kv_heads * head_dim, q.dtype)
+    dev = _kv4_device(op, q, k, v, positions, slots, inv_freq, cache, q_out)
+    pages, page = _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
+    dtype = q.dtype
+    code = _code(q, op)
+    q_stride = _kv4_rows(op, "q", q, None, num_heads * head_dim, dtype)
+    T = q.shape[0]
+    k_stride = _kv4_rows(op, "k", k, T, num_kv_heads * head_dim, dtype)
+    v_stride = _kv4_rows(op, "v", v, T, num_kv_heads * head_dim, dtype)
+    q_ptr = q.data_ptr()
+    out_ptr, out_stride = q_ptr, q_stride
     if q_out is not None:
-        _kv4_rows(op, "q_out", q_out, T, num_heads * head_dim, q.dtype)
-    q_out = q if q_out is None else q_out
+        out_ptr, out_stride = q_out.data_ptr(), _kv4_rows(op, "q_out", q_out, T, num_heads * head_dim, dtype)
     _int32_vec(positions, T, op, "positions")
     if slots is not None:
         _int32_vec(slots, T, op, "slots")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.shape != (head_dim // 2,) or not inv_freq.is_contiguous()):
+    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (head_dim // 2,) or not inv_freq.is_contiguous()):
         raise ShapeError(op, f"inv_freq must be float32 [{head_dim // 2}], got {inv_freq.dtype} {list(inv_freq.shape)}")
-    f = _fn("kv4", "vob_kv4_append", [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P])
-    _check(f(_ptr(q), q.stride(0), _ptr(q_out), q_out.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(positions), _ptr(slots),
-             _ptr(inv_freq), _ptr(cache), cache.shape[0], code, T, num_heads, num_kv_heads, head_dim, cache.shape[2], _stream()),
-           op, 1 if T else 0)
+    _check(_fn("kv4", "vob_kv4_append", _KV4_APPEND)(
+        q_ptr, q_stride, out_ptr, out_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, positions.data_ptr(),
+        None if slots is None else slots.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), cache.data_ptr(), pages, code, T,
+        num_heads, num_kv_heads, head_dim, page, _raw_stream(dev)), op, 1 if T else 0)
 
 
 @_timed
@@ -2305,16 +2333,15 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor, v_ou
     """The keys (as rotated) and values that a 4-bit cache holds at `slots` (int32 [T]), as numbers: k_out, v_out [T, KV*hd], float32
     or bfloat16. A negative slot gives zeros, one behind the pool NaN."""
     op = "kv4_read"
-    _cuda(op, cache, slots, k_out, v_out)
-    _kv4_cache(op, cache, num_kv_heads, num_kv_heads, head_dim)
-    _rows_2d(k_out, op, "k_out")
+    dev = _kv4_device(op, cache, slots, k_out, v_out)
+    pages, page = _kv4_cache(op, cache, num_kv_heads, num_kv_heads, head_dim)
+    code = _code(k_out, op)
+    k_stride = _kv4_rows(op, "k_out", k_out, None, num_kv_heads * head_dim, k_out.dtype)
     T = k_out.shape[0]
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        _kv4_rows(op, name, t, T, num_kv_heads * head_dim, k_out.dtype)
+    v_stride = _kv4_rows(op, "v_out", v_out, T, num_kv_heads * head_dim, k_out.dtype)
     _int32_vec(slots, T, op, "slots")
-    f = _fn("kv4", "vob_kv4_read", [_P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P])
-    _check(f(_ptr(cache), cache.shape[0], _ptr(slots), _ptr(k_out), k_out.stride(0), _ptr(v_out), v_out.stride(0), _code(k_out, op), T,
-             num_kv_heads, head_dim, cache.shape[2], _stream()), op, 1 if T else 0)
+    _check(_fn("kv4", "vob_kv4_read", _KV4_READ)(cache.data_ptr(), pages, slots.data_ptr(), k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride,
+                                                 code, T, num_kv_heads, head_dim, page, _raw_stream(dev)), op, 1 if T else 0)
 
 
 class KV4Scratch:
@@ -2324,6 +2351,7 @@ class KV4Scratch:
 
     def __init__(self, num_seqs: int, sizes: tuple, sms: int, partials: torch.Tensor, arrived: torch.Tensor):
         self.num_seqs, self.sizes, self.sms, self.partials, self.arrived = num_seqs, sizes, sms, partials, arrived
+        self.floats, self.counters = partials.numel(), arrived.numel()
 
 
 def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> KV4Scratch:
@@ -2339,21 +2367,20 @@ def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
 
 
 def _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window):
-    _cuda(op, q, out, cache, block_tables)
-    _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
-    _rows_2d(q, op, "q")
-    _code(q, op)
-    for name, t in (("q", q), ("out", out)):
-        _kv4_rows(op, name, t, q.shape[0], num_heads * head_dim, q.dtype)
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.shape[1] < 1:
+    """(type code, row strides of q and out, pages, page size, pages of a block table's row); `num_seqs` None: one per row of q."""
+    pages, page = _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
+    code = _code(q, op)
+    q_stride = _kv4_rows(op, "q", q, None, num_heads * head_dim, q.dtype)
+    rows = q.shape[0]
+    out_stride = _kv4_rows(op, "out", out, rows, num_heads * head_dim, q.dtype)
+    shape = block_tables.shape
+    if block_tables.dtype is not torch.int32 or len(shape) != 2 or not block_tables.is_contiguous() or shape[1] < 1:
         raise ShapeError(op, "block_tables must be contiguous int32 [S, max_pages]")
-    if block_tables.shape[0] < num_seqs:
-        raise ShapeError(op, f"block_tables has {block_tables.shape[0]} rows for {num_seqs} requests")
+    if shape[0] < (rows if num_seqs is None else num_seqs):
+        raise ShapeError(op, f"block_tables has {shape[0]} rows for {rows if num_seqs is None else num_seqs} requests")
     if window < 0:
         raise ShapeError(op, f"window {window} is negative")
-
-
-_KV4_ATTEND = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P]
+    return code, q_stride, out_stride, pages, page, shape[1]
 
 
 @_timed
@@ -2364,27 +2391,28 @@ def attn_decode_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     `scratch`: `kv4_scratch` for at least so many requests. A row whose page number lies outside the pool, or that sees a key or value
     kept as NaN, becomes NaN."""
     op = "attn_decode_kv4"
-    S = q.shape[0] if q.dim() == 2 else 0
-    _kv4_attn_checks(op, q, out, cache, block_tables, S, num_heads, num_kv_heads, head_dim, window)
-    _cuda(op, q, positions, scratch.partials, scratch.arrived)
+    partials, arrived = scratch.partials, scratch.arrived
+    dev = _kv4_device(op, q, out, cache, block_tables, positions, partials)
+    code, q_stride, out_stride, pages, page, max_pages = _kv4_attn_checks(op, q, out, cache, block_tables, None, num_heads, num_kv_heads, head_dim,
+                                                                          window)
+    S = q.shape[0]
     _int32_vec(positions, S, op, "positions")
     if scratch.sizes != (num_heads, num_kv_heads, head_dim) or S > scratch.num_seqs:
         raise ShapeError(op, f"the scratch was made for {scratch.num_seqs} requests of {scratch.sizes}, not for {S} of "
                              f"{(num_heads, num_kv_heads, head_dim)} (heads, kv heads, head size)")
-    sms, code = scratch.sms, _code(q, op)
-    if code == 1 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0:
-        f = _fn("kv4_decode", "vob_kv4_decode", [_P, _L, _P, _L, _P, _L, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P, _L, _I, _P, _P])
-        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
-                 _ptr(positions), S, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), _ptr(scratch.partials),
-                 scratch.partials.numel(), _ptr(scratch.arrived), scratch.arrived.numel(), sms, _ptr(_scratch_for(q.device).err), _stream()),
-               op, 1 if S else 0)
+    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    if code == 1 and q_stride % 8 == 0 and q_ptr % 16 == 0 and out_stride % 2 == 0 and out_ptr % 4 == 0:
+        _check(_fn("kv4_decode", "vob_kv4_decode", _KV4_DECODE)(
+            q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, positions.data_ptr(), S, num_heads,
+            num_kv_heads, head_dim, page, scale, window, partials.data_ptr(), scratch.floats, arrived.data_ptr(), scratch.counters, scratch.sms,
+            _scratch_for(q.device).err.data_ptr(), _raw_stream(dev)), op, 1 if S else 0)
         return
     # 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address
-    splits = max(1, min(32, 2 * sms // max(1, S * num_kv_heads * -(-(num_heads // num_kv_heads) // 16))))
-    f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
-    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
-             _ptr(positions), _P(0), _P(0), S, 1, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale), int(window), code,
-             splits, _ptr(scratch.partials), _ptr(scratch.arrived), _stream()), op, 1 if S else 0)
+    splits = max(1, min(32, 2 * scratch.sms // max(1, S * num_kv_heads * -(-(num_heads // num_kv_heads) // 16))))
+    _check(_fn("kv4", "vob_kv4_attend", _KV4_ATTEND)(
+        q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, positions.data_ptr(), None, None, S, 1,
+        num_heads, num_kv_heads, head_dim, page, scale, window, code, splits, partials.data_ptr(), arrived.data_ptr(), _raw_stream(dev)),
+        op, 1 if S else 0)
 
 
 @_timed
@@ -2396,22 +2424,25 @@ def attn_prefill_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, bl
     longest portion (a request's rows beyond it are not computed). `window` and what becomes NaN: as `attn_decode_kv4`. Rows that
     belong to no request are left as they are."""
     op = "attn_prefill_kv4"
-    _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window)
-    _cuda(op, q, seq_starts, context_lens)
+    dev = _kv4_device(op, q, out, cache, block_tables, seq_starts, context_lens)
+    code, q_stride, out_stride, pages, page, max_pages = _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim,
+                                                                          window)
     _int32_vec(seq_starts, num_seqs + 1, op, "seq_starts")
     _int32_vec(context_lens, num_seqs, op, "context_lens")
-    if (_code(q, op) == 1 and head_dim <= 128 and num_heads // num_kv_heads <= 128 and scale > 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
-            and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0):
-        f = _fn("kv4_prefill", "vob_kv4_prefill", [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P])
-        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
-                 _ptr(seq_starts), _ptr(context_lens), num_seqs, max_new, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale),
-                 int(window), _ptr(_scratch_for(q.device).err), _stream()), op, 1 if num_seqs > 0 and max_new > 0 else 0)
+    launches = 1 if num_seqs > 0 and max_new > 0 else 0
+    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    if (code == 1 and head_dim <= 128 and num_heads // num_kv_heads <= 128 and scale > 0 and q_stride % 8 == 0 and q_ptr % 16 == 0
+            and out_stride % 8 == 0 and out_ptr % 16 == 0):
+        _check(_fn("kv4_prefill", "vob_kv4_prefill", _KV4_PREFILL)(
+            q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, seq_starts.data_ptr(),
+            context_lens.data_ptr(), num_seqs, max_new, num_heads, num_kv_heads, head_dim, page, scale, window,
+            _scratch_for(q.device).err.data_ptr(), _raw_stream(dev)), op, launches)
         return
     # 32-bit arithmetic: the float32 engine, larger heads, and rows that the tensor-core kernel cannot address
-    f = _fn("kv4", "vob_kv4_attend", _KV4_ATTEND)
-    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(cache), cache.shape[0], _ptr(block_tables), block_tables.shape[1],
-             _P(0), _ptr(seq_starts), _ptr(context_lens), num_seqs, max_new, num_heads, num_kv_heads, head_dim, cache.shape[2], float(scale),
-             int(window), _code(q, op), 1, _P(0), _P(0), _stream()), op, 1 if num_seqs > 0 and max_new > 0 else 0)
+    _check(_fn("kv4", "vob_kv4_attend", _KV4_ATTEND)(
+        q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, None, seq_starts.data_ptr(),
+        context_lens.data_ptr(), num_seqs, max_new, num_heads, num_kv_heads, head_dim, page, scale, window, code, 1, None, None, _raw_stream(dev)),
+        op, launches)
 
 
 # ------------------------------------------------------------------------------------ sampling
