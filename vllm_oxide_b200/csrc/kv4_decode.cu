@@ -402,7 +402,7 @@ kv4_decode_kernel(const Args a) {
             }
             // below 2^-40 a scale counts as that: p itself stays below 2^55, whatever the values of the keys with large scores
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vt[i] = vs[i].x < 9.094947e-13f ? 9.094947e-13f : vs[i].x;
+            for (int i = 0; i < 4; ++i) vt[i] = fmaxf(vs[i].x, 9.094947e-13f);
             float p[2][NT][4], most = 0.f;                                           // the largest p_j times scale
             auto weigh = [&](int n) {
                 float e[4][2];
@@ -592,30 +592,67 @@ kv4_decode_kernel(const Args a) {
             __syncthreads();
             if (*s_last) {
                 __threadfence();
-                for (int i = threadIdx.x; i < Z::HEADS * 8 * NC; i += THREADS) {
-                    const int h = i / (8 * NC), d = 4 * (i % (8 * NC));
-                    if (h >= heads || d >= a.hd) continue;
+                // Eight parts of a thread on their way at once; where there are fewer numbers than threads, several threads share a number's parts. The
+                // order is fixed by the parts' places.
+                auto part_of = [&](int c) { return a.partials + (size_t)(2 * c + (share * c >= b0 ? 0 : 1)) * Z::PARTIAL; };
+                const int quads = a.hd / 4, items = heads * quads;
+                const int per = items > THREADS / 2 ? 1 : items > THREADS / 4 ? 2 : 4;
+                for (int i0 = 0; i0 < items; i0 += THREADS / per) {
+                    const int i = i0 + threadIdx.x / per;
+                    const bool mine = i < items;
+                    const int h = mine ? i / quads : 0, d = mine ? 4 * (i % quads) : 0;
                     float m = -INFINITY, sum = 0.f;
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* from = a.partials + (size_t)(2 * c + (share * c >= b0 ? 0 : 1)) * Z::PARTIAL;
-                        m = fmaxf(m, __ldcg(from + Z::HEADS * 32 * NC + h));
+                    for (int c = c0 + threadIdx.x % per; c <= c1; c += 8 * per) {
+                        float mc[8], lc[8];
+                        float4 v[8];
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            mc[b] = -INFINITY;
+                            lc[b] = 0.f;
+                            v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (c + b * per <= c1) {
+                                const float* from = part_of(c + b * per);
+                                mc[b] = __ldcg(from + Z::HEADS * 32 * NC + h);
+                                lc[b] = __ldcg(from + Z::HEADS * 32 * NC + Z::HEADS + h);
+                                v[b] = __ldcg(reinterpret_cast<const float4*>(from + h * (32 * NC) + d));
+                            }
+                        }
+                        float to = m;
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) to = fmaxf(to, mc[b]);
+                        float f = m == -INFINITY ? 1.f : exp2_fast(m - to);
+                        m = to;
+                        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+                        sum *= f;
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            // (a part whose keys all gave NaN has no reference: its sums are NaN and stay so)
+                            f = mc[b] == -INFINITY ? 1.f : exp2_fast(mc[b] - to);
+                            acc.x = fmaf(f, v[b].x, acc.x);
+                            acc.y = fmaf(f, v[b].y, acc.y);
+                            acc.z = fmaf(f, v[b].z, acc.z);
+                            acc.w = fmaf(f, v[b].w, acc.w);
+                            sum = fmaf(f, lc[b], sum);
+                        }
                     }
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* from = a.partials + (size_t)(2 * c + (share * c >= b0 ? 0 : 1)) * Z::PARTIAL;
-                        const float mc = __ldcg(from + Z::HEADS * 32 * NC + h);
-                        const float f = mc == -INFINITY ? 1.f : exp2_fast(mc - m);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + h * (32 * NC) + d));
-                        acc.x = fmaf(f, v.x, acc.x);
-                        acc.y = fmaf(f, v.y, acc.y);
-                        acc.z = fmaf(f, v.z, acc.z);
-                        acc.w = fmaf(f, v.w, acc.w);
-                        sum = fmaf(f, __ldcg(from + Z::HEADS * 32 * NC + Z::HEADS + h), sum);
+                    for (int off = 1; off < per; off <<= 1) {
+                        const float to = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off)), f = m == -INFINITY ? 1.f : exp2_fast(m - to);
+                        m = to;
+                        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+                        sum *= f;
+                        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+                        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+                        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+                        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, off);
                     }
-                    const float inv = 1.f / sum;
-                    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)at.s * a.out_stride + (size_t)(head0 + h) * a.hd + d);
-                    dst[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-                    dst[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                    if (mine && threadIdx.x % per == 0) {
+                        const float inv = 1.f / sum;
+                        __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)at.s * a.out_stride + (size_t)(head0 + h) * a.hd + d);
+                        dst[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+                        dst[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+                    }
                 }
             }
         }
