@@ -13,194 +13,303 @@ using namespace vob_kv4;
 //
 // A code is a decision: a key within a rounding of the border of two codes would land on either side, a whole step apart. So the
 // rotation of k is taken in 64 bits (sine and cosine once per token and pair, shared by all heads) and rounded to 32 bits
-// once; scale, minimum and codes are then fixed operations in 32 bits with one rounding each (no contraction into FMAs).
+// once; scale, minimum and codes are then fixed operations in 32 bits with one rounding each (no contraction into FMAs). A code's quotient is taken by a
+// reciprocal, and by a division where one of a lane's lies within 10^-5 of a border. q is rotated in 32 bits where it is bfloat16, in 64 where it is float32.
 //
-// One block per token (and per share of its vectors, where there are few tokens), eight warps that walk over its H + 2 G
-// vectors. LANES lanes hold a vector: unit u is the numbers 2u, 2u + 1 and their partners D/2 + 2u, D/2 + 2u + 1, that is one byte of codes in each half.
+// Sixteen lanes hold a vector (32 where it is longer than 128): lane l the Q numbers Ql ..., and their partners D/2 behind them, so a warp has two vectors at a time. A block of 8 warps
+// takes 2 tokens, four warps a token (where there are few, one token, and up to some blocks share it), so that what belongs to a token (its slot, the sines of a
+// lane's pairs) is looked up once. The loads of a warp are on their way together, before the sines are taken: with 32/8 heads of 128 it has 4 pairs of
+// queries and 2 of keys and values, 3 KB in flight.
 // Bound: memory (reads q, k, v once, writes q and 136 of 512 bytes per key and value at D = 128).
 // ---------------------------------------------------------------------------------------------
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_WARPS = 8;
 
-template <typename T> __device__ __forceinline__ float2 load2(const T* p, bool vec);
-template <> __device__ __forceinline__ float2 load2<float>(const float* p, bool vec) {
-    if (vec) return *reinterpret_cast<const float2*>(p);
-    return make_float2(p[0], p[1]);
-}
-template <> __device__ __forceinline__ float2 load2<__nv_bfloat16>(const __nv_bfloat16* p, bool vec) {
-    if (vec) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-    return make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
-}
-template <typename T> __device__ __forceinline__ void store2(T* p, float2 v, bool vec);
-template <> __device__ __forceinline__ void store2<float>(float* p, float2 v, bool vec) {
-    if (vec) *reinterpret_cast<float2*>(p) = v;
-    else { p[0] = v.x; p[1] = v.y; }
-}
-template <> __device__ __forceinline__ void store2<__nv_bfloat16>(__nv_bfloat16* p, float2 v, bool vec) {
-    if (vec) *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
-    else { p[0] = __float2bfloat16_rn(v.x); p[1] = __float2bfloat16_rn(v.y); }
-}
-
-__device__ __forceinline__ int code_of(float x, float m, float s) {
-    const float n = rintf(__fdiv_rn(__fsub_rn(x, m), s));
-    return (int)fminf(fmaxf(n, 0.f), 15.f);               // NaN (s is NaN): 0
-}
-
-// LANES lanes quantise one vector: lane `l` of them holds units l, l + LANES, ...: x[2i] the low pair, x[2i + 1] the high pair. Called by
-// whole warps (the reductions need every lane); vectors that are not kept have `store` false.
-template <int LANES, int UNITS>
-__device__ __forceinline__ void quantise_store(const float2 (&x)[2 * UNITS], int l, int hd, bool store, unsigned char* codes, int lane8,
-                                               uint32_t* params) {
-    const int units = hd >> 2;
-    float lo = INFINITY, hi = -INFINITY;
-    bool fin = true;
+// Q numbers of type T as 32-bit words.
+template <typename T, int Q> struct Words {
+    static constexpr int N = Q * (int)sizeof(T) / 4;
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (!vec) {
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i)
-        if (l + i * LANES < units) {
-            const float2 a = x[2 * i], b = x[2 * i + 1];
-            lo = fminf(lo, fminf(fminf(a.x, a.y), fminf(b.x, b.y)));
-            hi = fmaxf(hi, fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y)));
-            fin = fin && isfinite(a.x) && isfinite(a.y) && isfinite(b.x) && isfinite(b.y);
+            for (int i = 0; i < Q; i += 2) put2(i, ld_f(p + i), ld_f(p + i + 1));
+        } else if constexpr (N == 1) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (N == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+                w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+            }
         }
+    }
+    __device__ __forceinline__ void store(T* p, bool vec) const {
+        if (!vec) {
+#pragma unroll
+            for (int i = 0; i < Q; ++i) st_f(p + i, get(i));
+        } else if constexpr (N == 1) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else if constexpr (N == 2) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+    // numbers i and i + 1, i even
+    __device__ __forceinline__ void put2(int i, float x, float y) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(x);
+            w[i + 1] = __float_as_uint(y);
+        } else {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+            w[i / 2] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+};
+
+__device__ __forceinline__ float larger(float a, float b) {       // NaN if one of them is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float about_inverse(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// LANES lanes quantise a vector of which this lane has x[0 .. Q - 1] (numbers Ql ...) and x[Q ..] (D/2 behind them); `holds`: the lane has numbers.
+// Called by whole warps: the reductions need every lane.
+template <int Q, int LANES>
+__device__ __forceinline__ void quantise_store(const float (&x)[2 * Q], int l, int hd, bool holds, unsigned char* codes, int lane8,
+                                               uint32_t* params) {
+    float lo = INFINITY, hi = -INFINITY;
+    if (holds) {
+#pragma unroll
+        for (int i = 0; i < 2 * Q; ++i) {
+            lo = fminf(lo, x[i]);
+            hi = larger(hi, x[i]);
+        }
+    }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        fin = __shfl_xor_sync(0xffffffffu, (int)fin, o) && fin;
+        hi = larger(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    if (!store) return;
     const float fifteenth = 0.06666667014360428f;
     __nv_bfloat16 sb = __float2bfloat16_rn(__fsub_rn(__fmul_rn(hi, fifteenth), __fmul_rn(lo, fifteenth)));
     __nv_bfloat16 mb = __float2bfloat16_rn(lo);
+    const bool fin = hi < INFINITY && lo > -INFINITY;
     if (!fin) sb = mb = __float2bfloat16_rn(NAN);          // a vector with a number that is not finite is kept as NaN
     const float s = __bfloat162float(sb), m = __bfloat162float(mb);
-    const int last = 16 * chunks(hd);                      // bytes of codes, the rest of the last chunk included
+    if (holds) {
+        // u = (x - m) / 15 s, held to 0 .. 1; adding 1.5 2^23 to 15 u rounds to the nearest whole number, ties to even. u is off by at most 2^-22 of
+        // itself, 15 u by less than 4e-6: it is on the right side of a border that is 10^-5 away. (15 s is exact; outside 2^-100 .. 2^100 it is not
+        // tried.)
+        const bool plain = s > 7.888609e-31f && s < 1.2676506e30f;
+        const float inv = about_inverse(15.f * s);
+        float n[2 * Q], far = 0.f;
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const int u = l + i * LANES;
-        if (u < units) {
-            const float2 a = x[2 * i], b = x[2 * i + 1];
-            int na = 0, nb = 0;
-            if (s != 0.f) {
-                na = code_of(a.x, m, s) | code_of(a.y, m, s) << 4;
-                nb = code_of(b.x, m, s) | code_of(b.y, m, s) << 4;
-            }
-            const int ub = u + units;
-            codes[(u >> 4) * 128 + lane8 * 16 + (u & 15)] = (unsigned char)na;
-            codes[(ub >> 4) * 128 + lane8 * 16 + (ub & 15)] = (unsigned char)nb;
+        for (int i = 0; i < 2 * Q; ++i) {
+            const float u = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv));
+            n[i] = __fsub_rn(fmaf(u, 15.f, 12582912.f), 12582912.f);
+            far = fmaxf(far, fabsf(fmaf(u, 15.f, -n[i])));
+        }
+        if (!plain || far > 0.49999f) {
+#pragma unroll
+            for (int i = 0; i < 2 * Q; ++i) n[i] = s != 0.f && fin ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], m), s)), 0.f), 15.f) : 0.f;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const float* c = n + half * Q;
+            uint32_t packed;                               // sums of codes times powers of 16: whole numbers below 2^16, exact
+            if constexpr (Q == 2) packed = (uint32_t)fmaf(c[1], 16.f, c[0]);
+            else packed = (uint32_t)fmaf(fmaf(c[3], 16.f, c[2]), 256.f, fmaf(c[1], 16.f, c[0]));
+            const int b = l * (Q / 2) + half * (hd >> 2);  // the first byte of codes, of all the vector's
+            unsigned char* at = codes + (b >> 4) * 128 + lane8 * 16 + (b & 15);
+            if constexpr (Q == 2) *at = (unsigned char)packed;
+            else *reinterpret_cast<unsigned short*>(at) = (unsigned short)packed;
         }
     }
-    const int tail = 2 * units + l;                        // the rest of the last chunk: at most 8 bytes (head sizes are multiples of 16)
-    if (tail < last) codes[(tail >> 4) * 128 + lane8 * 16 + (tail & 15)] = 0;
+    const int tail = (hd >> 1) + l;                        // the rest of the last chunk: 8 bytes at most (head sizes are multiples of 16)
+    if (tail < 16 * chunks(hd)) codes[(tail >> 4) * 128 + lane8 * 16 + (tail & 15)] = 0;
     if (l == 0) *params = (uint32_t)__bfloat16_as_ushort(sb) | (uint32_t)__bfloat16_as_ushort(mb) << 16;
 }
 
-template <typename T, int LANES, int UNITS>
-__global__ void __launch_bounds__(APPEND_THREADS)
-kv4_append_kernel(const T* q, long long q_stride, T* q_out, long long qo_stride, const T* __restrict__ k, long long k_stride,
-                  const T* __restrict__ v, long long v_stride, const int* __restrict__ positions, const int* __restrict__ slots,
-                  const float* __restrict__ inv_freq, unsigned char* __restrict__ cache, long long num_slots, int H, int G, int hd,
-                  int page_size, bool vec) {
-    __shared__ double2 turn[128];                          // cosine and sine of the token's angles
+struct AppendArgs {
+    const void *q, *k, *v;
+    void* q_out;
+    long long q_stride, qo_stride, k_stride, v_stride;
+    const int *positions, *slots;
+    const float* inv_freq;
+    unsigned char* cache;
+    long long num_slots;
+    int T, H, G, hd, page_size;
+    bool vec;
+};
+
+template <typename T, int Q, int LANES, int TOKENS>
+__global__ void __launch_bounds__(32 * APPEND_WARPS, 2)
+kv4_append_kernel(const AppendArgs a) {
+    constexpr int HALF = LANES * Q;                        // most pairs of a vector: head sizes up to 64, 128, 256
+    constexpr int WORDS = Words<T, Q>::N;
+    constexpr int QB = TOKENS == 1 ? 1 : WORDS <= 2 ? 4 : 2, KB = TOKENS == 1 ? 1 : QB / 2;    // pairs of vectors loaded at a time
+    constexpr bool FLOAT_Q = sizeof(T) == 2;
+    __shared__ double2 turn[TOKENS][HALF];                 // cosine and sine of the tokens' angles
     pdl_launch_dependents();
     pdl_wait(30);
-    const int t = blockIdx.x, half = hd >> 1;
-    if (inv_freq) {
-        const float pos = (float)positions[t];
-        for (int i = threadIdx.x; i < half; i += APPEND_THREADS) {
-            const float theta = pos * inv_freq[i];
-            double s, c;
-            sincospi((double)theta * 0.31830988618379067154, &s, &c);
-            turn[i] = make_double2(c, s);
-        }
-    } else {
-        for (int i = threadIdx.x; i < half; i += APPEND_THREADS) turn[i] = make_double2(1.0, 0.0);
-    }
-    __syncthreads();
-    const int slot = slots ? slots[t] : -1;
-    const bool keep = slot >= 0 && slot < num_slots;
-    const int page = keep ? slot / page_size : 0, off = keep ? slot - page * page_size : 0;
-    const int C = chunks(hd), width = token_bytes(hd), units = hd >> 2;
-    constexpr int PER_WARP = 32 / LANES;                   // vectors a warp works on side by side
-    const int l = threadIdx.x % LANES;
-    const int first = (blockIdx.y * (APPEND_THREADS / 32) + (threadIdx.x >> 5)) * PER_WARP + (threadIdx.x & 31) / LANES;
-    const int step = gridDim.y * (APPEND_THREADS / 32) * PER_WARP;
-    const int vectors = H + 2 * G;
-    // every lane of a warp takes part in the reductions: the loop runs as long as one of its vectors is there
-    for (int e0 = first - (threadIdx.x & 31) / LANES; e0 < vectors; e0 += step) {
-        const int e = e0 + (threadIdx.x & 31) / LANES;
-        const bool is_q = e < H, is_k = !is_q && e < H + G, there = e < vectors;
-        const int head = is_q ? e : is_k ? e - H : e - H - G;
-        const T* src = is_q ? q + (size_t)t * q_stride : is_k ? k + (size_t)t * k_stride : v + (size_t)t * v_stride;
-        src += (size_t)head * hd;
-        float2 x[2 * UNITS];
+    const int warp = threadIdx.x >> 5, l = threadIdx.x % LANES, sub = (threadIdx.x & 31) / LANES;
+    constexpr int AT_ONCE = 32 / LANES;                    // vectors of a warp
+    constexpr int PER_BLOCK = APPEND_WARPS / TOKENS;       // warps of a block that share a token
+    const int mine = warp / PER_BLOCK, t = blockIdx.x * TOKENS + mine, half = a.hd >> 1;
+    const int sharers = PER_BLOCK * gridDim.y, me = blockIdx.y * PER_BLOCK + warp % PER_BLOCK;
+    const bool holds = l * Q < half, live = t < a.T;
+    // pairs (AT_ONCE) of queries from the first warp on, of keys and values from the last
+    const int q_pairs = (a.H + AT_ONCE - 1) / AT_ONCE, kv_pairs = 2 * a.G / AT_ONCE, kv_me = sharers - 1 - me;
+
+    Words<T, Q> rq[QB][2], rk[KB][2];
+    auto load = [&](int round) {
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            const int u = l + i * LANES;
-            x[2 * i] = x[2 * i + 1] = make_float2(0.f, 0.f);
-            if (there && u < units) {
-                float2 a = load2(src + 2 * u, vec), b = load2(src + half + 2 * u, vec);
-                if (is_q || is_k) {
-                    const double2 t0 = turn[2 * u], t1 = turn[2 * u + 1];
-                    const double ax = a.x, ay = a.y, bx = b.x, by = b.y;
-                    a = make_float2((float)(ax * t0.x - bx * t0.y), (float)(ay * t1.x - by * t1.y));
-                    b = make_float2((float)(bx * t0.x + ax * t0.y), (float)(by * t1.x + ay * t1.y));
+        for (int b = 0; b < QB; ++b) {
+            const int e = AT_ONCE * (me + (round * QB + b) * sharers) + sub;
+            if (!live || !holds || e >= a.H) continue;
+            const T* src = (const T*)a.q + (size_t)t * a.q_stride + e * a.hd + l * Q;
+            rq[b][0].load(src, a.vec);
+            rq[b][1].load(src + half, a.vec);
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int e = AT_ONCE * (kv_me + (round * KB + b) * sharers) + sub;
+            if (!live || !holds || e >= 2 * a.G) continue;
+            const T* src = (e < a.G ? (const T*)a.k + (size_t)t * a.k_stride + e * a.hd : (const T*)a.v + (size_t)t * a.v_stride + (e - a.G) * a.hd) + l * Q;
+            rk[b][0].load(src, a.vec);
+            rk[b][1].load(src + half, a.vec);
+        }
+    };
+    load(0);
+    for (int i = threadIdx.x; i < TOKENS * HALF; i += 32 * APPEND_WARPS) {
+        const int tt = i / HALF, p = i % HALF;
+        double s = 0.0, c = 1.0;
+        if (a.inv_freq && p < half && blockIdx.x * TOKENS + tt < a.T) {
+            const float theta = (float)a.positions[blockIdx.x * TOKENS + tt] * a.inv_freq[p];
+            sincospi((double)theta * 0.31830988618379067154, &s, &c);
+        }
+        turn[tt][p] = make_double2(c, s);
+    }
+    const int slot = live && a.slots ? a.slots[t] : -1;
+    __syncthreads();
+    if (!live) return;
+    const bool keep = slot >= 0 && slot < a.num_slots;
+    const int page = keep ? slot / a.page_size : 0, off = keep ? slot - page * a.page_size : 0;
+    const int C = chunks(a.hd), width = token_bytes(a.hd);
+    unsigned char* groups = a.cache + group_at(page, 0, off, a.G, a.page_size, width);     // of kv head 0; the others follow at equal distances
+    const size_t next_head = (size_t)a.page_size * width;
+    float2 cs[FLOAT_Q ? Q : 1];
+    if constexpr (FLOAT_Q) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const double2 v = turn[mine][l * Q + i];
+            cs[i] = make_float2((float)v.x, (float)v.y);
+        }
+    }
+    for (int round = 0;; ++round) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            const int e = AT_ONCE * (me + (round * QB + b) * sharers) + sub;
+            if (!holds || e >= a.H) continue;
+            Words<T, Q> r0, r1;
+#pragma unroll
+            for (int i = 0; i < Q; i += 2) {
+                float lo[2], hi[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float x = rq[b][0].get(i + j), y = rq[b][1].get(i + j);
+                    if constexpr (FLOAT_Q) {
+                        lo[j] = x * cs[i + j].x - y * cs[i + j].y;
+                        hi[j] = y * cs[i + j].x + x * cs[i + j].y;
+                    } else {
+                        const double2 v = turn[mine][l * Q + i + j];
+                        lo[j] = (float)((double)x * v.x - (double)y * v.y);
+                        hi[j] = (float)((double)y * v.x + (double)x * v.y);
+                    }
                 }
-                x[2 * i] = a;
-                x[2 * i + 1] = b;
-                if (is_q) {
-                    T* dst = q_out + (size_t)t * qo_stride + (size_t)head * hd;
-                    store2(dst + 2 * u, a, vec);
-                    store2(dst + half + 2 * u, b, vec);
+                r0.put2(i, lo[0], lo[1]);
+                r1.put2(i, hi[0], hi[1]);
+            }
+            T* dst = (T*)a.q_out + (size_t)t * a.qo_stride + e * a.hd + l * Q;
+            r0.store(dst, a.vec);
+            r1.store(dst + half, a.vec);
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int pair = kv_me + (round * KB + b) * sharers;
+            if (!keep || pair >= kv_pairs) break;          // (the token's slot and the pair are the warp's)
+            const int e = AT_ONCE * pair + sub;
+            const bool is_k = e < a.G;
+            float x[2 * Q];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                x[i] = rk[b][0].get(i);
+                x[Q + i] = rk[b][1].get(i);
+                if (is_k && holds) {
+                    const double2 v = turn[mine][l * Q + i];
+                    const double p = x[i], q = x[Q + i];
+                    x[i] = (float)(p * v.x - q * v.y);
+                    x[Q + i] = (float)(q * v.x + p * v.y);
                 }
             }
+            unsigned char* group = groups + (is_k ? e : e - a.G) * next_head;
+            quantise_store<Q, LANES>(x, l, a.hd, holds, group + (is_k ? 0 : 128 * C), off & 7,
+                              reinterpret_cast<uint32_t*>(group + 256 * C) + 2 * (off & 7) + (is_k ? 0 : 1));
         }
-        const bool store = there && !is_q && keep;
-        if (__any_sync(0xffffffffu, store)) {
-            unsigned char* group = cache + group_at(page, head, off, G, page_size, width);
-            unsigned char* codes = group + (is_k ? 0 : 128 * C);
-            uint32_t* params = reinterpret_cast<uint32_t*>(group + 256 * C) + 2 * (off & 7) + (is_k ? 0 : 1);
-            quantise_store<LANES, UNITS>(x, l, hd, store, codes, off & 7, params);
-        }
+        if (me + (round + 1) * QB * sharers >= q_pairs && kv_me + (round + 1) * KB * sharers >= kv_pairs) break;
+        load(round + 1);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Read back: the keys and values that the cache holds at the given slots, m + s n rounded once to the outputs' type.
-// A negative slot gives zeros, one behind the pool NaN. One thread per row, kv head and 4 numbers of the key and of the value. Bound: memory.
+// A negative slot gives zeros, one behind the pool NaN. A block per row, a thread per 8 numbers of a head's key and value. Bound: memory.
 // ---------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const unsigned char* __restrict__ cache, long long num_slots, const int* __restrict__ slots, T* __restrict__ k_out,
-                long long k_stride, T* __restrict__ v_out, long long v_stride, long long items, int G, int hd, int page_size) {
+                long long k_stride, T* __restrict__ v_out, long long v_stride, int G, int hd, int page_size, bool vec) {
     pdl_launch_dependents();
     pdl_wait(31);
-    const int quads = hd >> 2, C = chunks(hd);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < items; i += (long long)gridDim.x * 256) {
-        const int u = (int)(i % quads);
-        const long long rh = i / quads;
-        const int head = (int)(rh % G);
-        const long long t = rh / G;
-        const int slot = slots[t];
-        float kv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (slot >= num_slots) {
-            for (int j = 0; j < 8; ++j) kv[j] = NAN;
+    const int t = blockIdx.x, slot = slots[t], words = hd >> 3, C = chunks(hd), width = token_bytes(hd);
+    const bool there = slot >= 0 && slot < num_slots;
+    const int page = there ? slot / page_size : 0, off = there ? slot - page * page_size : 0;
+    const unsigned char* groups = cache + group_at(page, 0, off, G, page_size, width);
+    for (int i = threadIdx.x; i < G * words; i += 256) {
+        const int head = i / words, u = i - head * words;
+        const unsigned char* group = groups + (size_t)head * page_size * width;
+        uint2 par = make_uint2(0, 0);
+        uint32_t n[2] = {0, 0};
+        if (there) {
+            par = *reinterpret_cast<const uint2*>(group + 256 * C + 8 * (off & 7));
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                n[w] = *reinterpret_cast<const uint32_t*>(group + (w * C + (u >> 2)) * 128 + (off & 7) * 16 + (u & 3) * 4);
         } else if (slot >= 0) {
-            const int page = slot / page_size, off = slot - page * page_size;
-            const unsigned char* group = cache + group_at(page, head, off, G, page_size, token_bytes(hd));
-            const int at = (u >> 3) * 128 + (off & 7) * 16 + (u & 7) * 2;
-            const uint2 p = *reinterpret_cast<const uint2*>(group + 256 * C + 8 * (off & 7));
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const unsigned short n = *reinterpret_cast<const unsigned short*>(group + w * 128 * C + at);
-                const float2 sm = scale_min(w ? p.y : p.x);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) kv[4 * w + j] = fmaf((float)(n >> (4 * j) & 15), sm.x, sm.y);
-            }
+            par = make_uint2(0x7fff7fffu, 0x7fff7fffu);
         }
-        T* ko = k_out + t * k_stride + (size_t)head * hd + 4 * u;
-        T* vo = v_out + t * v_stride + (size_t)head * hd + 4 * u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { st_f(ko + j, kv[j]); st_f(vo + j, kv[4 + j]); }
+        for (int w = 0; w < 2; ++w) {
+            const float2 sm = scale_min(w ? par.y : par.x);
+            Words<T, 8> out;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                out.put2(j, fmaf((float)(n[w] >> (4 * j) & 15), sm.x, sm.y), fmaf((float)(n[w] >> (4 * j + 4) & 15), sm.x, sm.y));
+            out.store((w ? v_out + (size_t)t * v_stride : k_out + (size_t)t * k_stride) + head * hd + 8 * u, vec);
+        }
     }
 }
 
@@ -465,23 +574,24 @@ VOB_EXPORT int vob_kv4_append(const void* q, long long q_stride, void* q_out, lo
                               void* cache, long long num_pages, int code, int T, int H, int G, int hd, int page_size, cudaStream_t stream) {
     if (T <= 0) return 0;
     if (!sizes_ok(H, G, hd, page_size) || num_pages <= 0) return VOB_ERR_BAD_ARG;
-    const int es = code == VOB_F32 ? 4 : 2;
-    const bool vec = (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) % (2 * es)) == 0 &&
-                     ((q_stride | qo_stride | k_stride | v_stride) % 2) == 0;
-    const long long num_slots = num_pages * page_size;
-    const int vectors = H + 2 * G, lanes = hd <= 64 ? 16 : 32;
-    const int per_pass = (APPEND_THREADS / 32) * (32 / lanes);
-    // few tokens: a block per pass over the vectors, so that a decode step's tokens spread over the GPU
-    int y = (vectors + per_pass - 1) / per_pass;
-    if ((long long)T * y > 4 * 148) y = (int)max(1LL, (long long)(4 * 148) / T);
-    const dim3 grid(T, y), block(APPEND_THREADS);
-#define VOB_APPEND(L, U)                                                                                                              \
-    VOB_DISPATCH_ELEM(code, return vob_launch(kv4_append_kernel<ElemT, L, U>, grid, block, 0, stream, (const ElemT*)q, q_stride,          \
-                                              (ElemT*)q_out, qo_stride, (const ElemT*)k, k_stride, (const ElemT*)v, v_stride, positions,  \
-                                              slots, inv_freq, (unsigned char*)cache, num_slots, H, G, hd, page_size, vec))
-    if (hd <= 64) VOB_APPEND(16, 1);
-    if (hd <= 128) VOB_APPEND(32, 1);
-    VOB_APPEND(32, 2);
+    // Q numbers a lane, which are loaded at once where rows allow it
+    const int Q = hd <= 64 ? 2 : 4, at = Q * (code == VOB_F32 ? 4 : 2), at_once = hd <= 128 ? 2 : 1;
+    const bool vec = (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) % at) == 0 &&
+                     ((q_stride | qo_stride | k_stride | v_stride) % Q) == 0;
+    const AppendArgs a = {q, k, v, q_out, q_stride, qo_stride, k_stride, v_stride, positions, slots, inv_freq, (unsigned char*)cache,
+                          num_pages * page_size, T, H, G, hd, page_size, vec};
+    // up to three blocks an SM a token has a block, and several where its vectors are enough for them, so that a decode step spreads over the GPU
+    const bool few = T <= 148 * 3;
+    const int wanted = ((H + at_once - 1) / at_once + 2 * G / at_once + APPEND_WARPS - 1) / APPEND_WARPS;
+    const dim3 grid(few ? T : (T + 1) / 2, few ? max(1, min(wanted, 148 * 3 / T)) : 1), block(32 * APPEND_WARPS);
+#define VOB_APPEND(Q, L)                                                                                           \
+    do {                                                                                                           \
+        if (few) VOB_DISPATCH_ELEM(code, return vob_launch(kv4_append_kernel<ElemT, Q, L, 1>, grid, block, 0, stream, a)); \
+        VOB_DISPATCH_ELEM(code, return vob_launch(kv4_append_kernel<ElemT, Q, L, 2>, grid, block, 0, stream, a));          \
+    } while (0)
+    if (hd <= 64) VOB_APPEND(2, 16);
+    if (hd <= 128) VOB_APPEND(4, 16);
+    VOB_APPEND(4, 32);
 #undef VOB_APPEND
     return 0;
 }
@@ -490,11 +600,9 @@ VOB_EXPORT int vob_kv4_read(const void* cache, long long num_pages, const int* s
                             long long v_stride, int code, int T, int G, int hd, int page_size, cudaStream_t stream) {
     if (T <= 0) return 0;
     if (!sizes_ok(G, G, hd, page_size) || num_pages <= 0) return VOB_ERR_BAD_ARG;
-    const long long items = (long long)T * G * (hd >> 2);
-    const long long blocks = (items + 255) / 256;
-    VOB_DISPATCH_ELEM(code, return vob_launch(kv4_read_kernel<ElemT>, dim3((unsigned)min(blocks, 148LL * 16)), dim3(256), 0, stream,
-                                              (const unsigned char*)cache, num_pages * page_size, slots, (ElemT*)k_out, k_stride,
-                                              (ElemT*)v_out, v_stride, items, G, hd, page_size));
+    const bool vec = (((uintptr_t)k_out | (uintptr_t)v_out) % 16) == 0 && ((k_stride | v_stride) % 8) == 0;
+    VOB_DISPATCH_ELEM(code, return vob_launch(kv4_read_kernel<ElemT>, dim3(T), dim3(256), 0, stream, (const unsigned char*)cache,
+                                              num_pages * page_size, slots, (ElemT*)k_out, k_stride, (ElemT*)v_out, v_stride, G, hd, page_size, vec));
     return 0;
 }
 
