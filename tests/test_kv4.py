@@ -27,23 +27,9 @@ def test_packing_all_at_once_and_one_by_one_make_the_same_bytes(hd, page):
     assert (off <= 0.5 * s.double()[..., None] * (1 + 1e-6) + 2.0 ** -8 * (15 * s.abs() + m.abs()).double()[..., None]).all()
 
 
-def test_there_is_no_cpu_path():
-    c = torch.zeros(2, 1, 8, kernels.kv4_width(16), dtype=torch.uint8)
-    x, i = torch.zeros(1, 16), torch.zeros(1, dtype=torch.int32)
-    with pytest.raises(KernelError):
-        kernels.kv4_append(x, x, x, i, i, None, c, 1, 1, 16)
-    with pytest.raises(KernelError):
-        kernels.kv4_read(c, i, x, x, 1, 16)
-
-
 @pytest.fixture
 def no_gpu(monkeypatch):
-    """The wrappers' checks on CPU tensors: the device's check passes, a launch is a failure."""
-    monkeypatch.setattr(kernels, "_kv4_device", lambda *a: 0)
-
-    def launch(*a):
-        raise AssertionError("a launch was reached")
-    monkeypatch.setattr(kernels, "_fn", launch)
+    """Shapes, types and strides are checked before devices: what does not fit is refused wherever the tensors are."""
     monkeypatch.setattr(torch.cuda, "get_device_properties", lambda d: type("P", (), {"multi_processor_count": 148})())
 
 
@@ -103,6 +89,19 @@ def test_portions_refuse(no_gpu, change):
     a.update(change)
     with pytest.raises(ShapeError):
         kernels.attn_prefill_kv4(**a)
+
+
+def test_there_is_no_cpu_path(no_gpu):
+    """Calls that fit, on the CPU."""
+    c = torch.zeros(2, 1, 8, kernels.kv4_width(16), dtype=torch.uint8)
+    x, i, t = torch.zeros(1, 16), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    for call in (lambda: kernels.kv4_append(x, x, x, i, i, None, c, 1, 1, 16), lambda: kernels.kv4_read(c, i, x, x, 1, 16),
+                 lambda: kernels.attn_decode_kv4(x, x, c, t, i, 1, 1, 16, 1.0, scratch=kernels.kv4_scratch(1, 1, 1, 16, "cpu")),
+                 lambda: kernels.attn_prefill_kv4(x, x, c, t, torch.zeros(2, dtype=torch.int32), i, 1, 1, 1, 1, 16, 1.0),
+                 lambda: kernels.kv4_append(**_append_args()), lambda: kernels.kv4_append(**_append_args(q_out=torch.zeros(3, 128), slots=None)),
+                 lambda: kernels.kv4_append(**_append_args(q=torch.zeros(3, 300)[:, 9:137], inv_freq=None))):
+        with pytest.raises(KernelError, match="no CPU path"):
+            call()
 
 
 def test_scratch_refuses(no_gpu):

@@ -1,7 +1,8 @@
-// Python bindings of the host runtime: cache manager, step-batch builder, scheduler.
+// Python bindings of the host runtime: cache manager, step-batch builder, scheduler, the calls of the 4-bit cache's operators.
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <pybind11/numpy.h>
+#include "kv4_calls.h"
 #include "scheduler.h"
 
 namespace py = pybind11;
@@ -152,4 +153,6 @@ PYBIND11_MODULE(VOB_MODULE_NAME, m) {
         .def("tokens_of", [](const Scheduler& s, int64_t id) { return s.request(id).tokens; })
         .def("computed_of", [](const Scheduler& s, int64_t id) { return s.request(id).computed; })
         .def("preemptions_of", [](const Scheduler& s, int64_t id) { return s.request(id).preemptions; });
+
+    if (PyModule_AddFunctions(m.ptr(), vob_calls::methods())) throw py::error_already_set();
 }

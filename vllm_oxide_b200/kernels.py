@@ -2248,52 +2248,39 @@ def kv4_supported(num_heads: int, num_kv_heads: int, head_dim: int, page_size: i
             and page_size > 0 and page_size % 8 == 0)
 
 
-# The wrappers below are called once or more per layer of a decode step whose kernels take some microseconds: their checks read each of a
-# tensor's properties once, and pointers go to ctypes as plain integers.
-def _kv4_device(op, *tensors) -> int:
-    """The current device, on which all of the tensors must be (launches go to its current stream)."""
-    first = tensors[0].get_device()
-    dev = torch._C._cuda_getDevice() if first >= 0 else -1
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or first < 0):
-            _cuda(op, *tensors)
-            raise ShapeError(op, f"the tensors are on {t.device}, the current device is cuda:{dev}: launches go to its stream")
-    return dev
+# The calls of this cache are made by the native runtime (csrc/runtime/kv4_calls.h): its checks of every shape, type, stride, device and alignment take
+# half a microsecond a tensor less than here, which is what such a call of a decode step is made of.
+_kv4_native = None
 
 
-def _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim):
-    """(pages, page size) of a cache that fits."""
-    shape = cache.shape
-    if cache.dtype is not torch.uint8 or len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != 32 * -(-head_dim // 32) + 8 \
-            or not cache.is_contiguous() or shape[0] < 1:
-        raise ShapeError(op, f"the cache must be contiguous uint8 [pages, {num_kv_heads}, page_size, {kv4_width(head_dim)}], got "
-                             f"{cache.dtype} {list(shape)}")
-    pages, page = shape[0], shape[2]
-    if pages * page > 2 ** 31 - 1:
-        raise ShapeError(op, f"{pages} pages of {page} tokens are beyond 2^31 - 1 slots")
-    if cache.data_ptr() % 16:
-        raise ShapeError(op, "the cache must start on a 16-byte boundary")
-    if not kv4_supported(num_heads, num_kv_heads, head_dim, page):
-        raise ShapeError(op, f"sizes not supported: heads {num_heads}/{num_kv_heads}, head_dim {head_dim} (multiples of 16 up to 256), "
-                             f"page {page} (multiples of 8)")
-    return pages, page
+class _KV4Calls:
+    """The native calls and the addresses of the kernels' entry points (0 where there is no CUDA device: no call gets that far)."""
+
+    def __init__(self):
+        from .csrc.build import runtime_module
+        rt = runtime_module()
+        rt.kv4_setup(ShapeError, KernelError, torch.float32, torch.bfloat16, torch.uint8, torch.int32,
+                     getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None))
+        self.append, self.read, self.decode, self.prefill = rt.kv4_append, rt.kv4_read, rt.attn_decode_kv4, rt.attn_prefill_kv4
+
+        def entry(module, name):
+            return ctypes.cast(getattr(_load(module), name), _P).value if torch.cuda.is_available() else 0
+        self.append_entry, self.read_entry, self.attend_entry = (entry("kv4", "vob_kv4_" + n) for n in ("append", "read", "attend"))
+        self.decode_entry, self.prefill_entry = entry("kv4_decode", "vob_kv4_decode"), entry("kv4_prefill", "vob_kv4_prefill")
 
 
-def _kv4_rows(op, name, t, rows, cols, dtype) -> int:
-    """The row stride of a [rows, cols] tensor of this type with unit inner stride (`rows` None: any number)."""
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 2 or (rows is not None and shape[0] != rows) or shape[1] != cols or t.dtype is not dtype or strides[1] != 1:
-        raise ShapeError(op, f"{name} must be {dtype} [{'T' if rows is None else rows}, {cols}] with unit inner stride, got {t.dtype} {list(shape)} "
-                             f"strides {list(strides)}")
-    return strides[0]
+def _kv4() -> _KV4Calls:
+    global _kv4_native
+    if _kv4_native is None:
+        _kv4_native = _KV4Calls()
+    return _kv4_native
 
 
-_KV4_APPEND = [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P]
-_KV4_READ = [_P, _L, _P, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P]
-_KV4_ATTEND = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P]
-_KV4_DECODE = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I, _P, _L, _P, _L, _I, _P, _P]
-_KV4_PREFILL = [_P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P]
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _kv4_done(status: int, op: str) -> None:
+    if status:
+        _check(max(status, 0), op, 0)              # -1: there was nothing to launch
+    else:
+        count_launches(1)
 
 
 @_timed
@@ -2304,44 +2291,16 @@ def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     in 4 bits at their slots of `cache` (one layer's pages, see `kv4_width`). q [T, H*hd], k and v [T, KV*hd] may be column slices of one
     wider tensor; k and v are left as they are. A token whose slot is negative (or `slots` None, or a slot behind the pool) is not
     kept; no two tokens of one call may have the same slot. A key or value with a number that is not finite is kept as NaN."""
-    op = "kv4_append"
-    dev = _kv4_device(op, q, k, v, positions, slots, inv_freq, cache, q_out)
-    pages, page = _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
-    dtype = q.dtype
-    code = _code(q, op)
-    q_stride = _kv4_rows(op, "q", q, None, num_heads * head_dim, dtype)
-    T = q.shape[0]
-    k_stride = _kv4_rows(op, "k", k, T, num_kv_heads * head_dim, dtype)
-    v_stride = _kv4_rows(op, "v", v, T, num_kv_heads * head_dim, dtype)
-    q_ptr = q.data_ptr()
-    out_ptr, out_stride = q_ptr, q_stride
-    if q_out is not None:
-        out_ptr, out_stride = q_out.data_ptr(), _kv4_rows(op, "q_out", q_out, T, num_heads * head_dim, dtype)
-    _int32_vec(positions, T, op, "positions")
-    if slots is not None:
-        _int32_vec(slots, T, op, "slots")
-    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (head_dim // 2,) or not inv_freq.is_contiguous()):
-        raise ShapeError(op, f"inv_freq must be float32 [{head_dim // 2}], got {inv_freq.dtype} {list(inv_freq.shape)}")
-    _check(_fn("kv4", "vob_kv4_append", _KV4_APPEND)(
-        q_ptr, q_stride, out_ptr, out_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, positions.data_ptr(),
-        None if slots is None else slots.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), cache.data_ptr(), pages, code, T,
-        num_heads, num_kv_heads, head_dim, page, _raw_stream(dev)), op, 1 if T else 0)
+    n = _kv4_native or _kv4()
+    _kv4_done(n.append(n.append_entry, q, k, v, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, q_out), "kv4_append")
 
 
 @_timed
 def kv4_read(cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
     """The keys (as rotated) and values that a 4-bit cache holds at `slots` (int32 [T]), as numbers: k_out, v_out [T, KV*hd], float32
     or bfloat16. A negative slot gives zeros, one behind the pool NaN."""
-    op = "kv4_read"
-    dev = _kv4_device(op, cache, slots, k_out, v_out)
-    pages, page = _kv4_cache(op, cache, num_kv_heads, num_kv_heads, head_dim)
-    code = _code(k_out, op)
-    k_stride = _kv4_rows(op, "k_out", k_out, None, num_kv_heads * head_dim, k_out.dtype)
-    T = k_out.shape[0]
-    v_stride = _kv4_rows(op, "v_out", v_out, T, num_kv_heads * head_dim, k_out.dtype)
-    _int32_vec(slots, T, op, "slots")
-    _check(_fn("kv4", "vob_kv4_read", _KV4_READ)(cache.data_ptr(), pages, slots.data_ptr(), k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride,
-                                                 code, T, num_kv_heads, head_dim, page, _raw_stream(dev)), op, 1 if T else 0)
+    n = _kv4_native or _kv4()
+    _kv4_done(n.read(n.read_entry, cache, slots, k_out, v_out, num_kv_heads, head_dim), "kv4_read")
 
 
 class KV4Scratch:
@@ -2349,9 +2308,9 @@ class KV4Scratch:
     calls. The counters are zero between launches. Launches that use the same one must not run at the same time: one per stream,
     and graphs that share one are replayed one behind the other."""
 
-    def __init__(self, num_seqs: int, sizes: tuple, sms: int, partials: torch.Tensor, arrived: torch.Tensor):
-        self.num_seqs, self.sizes, self.sms, self.partials, self.arrived = num_seqs, sizes, sms, partials, arrived
-        self.floats, self.counters = partials.numel(), arrived.numel()
+    def __init__(self, made_for: tuple, sms: int, partials: torch.Tensor, arrived: torch.Tensor, err: torch.Tensor):
+        self.made_for, self.sms, self.partials, self.arrived = made_for, sms, partials, arrived     # (requests, heads, kv heads, head size)
+        self.err, self.err_ptr = err, err.data_ptr()
 
 
 def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> KV4Scratch:
@@ -2362,25 +2321,9 @@ def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
     # two partial results per block; at most 48 heads in the blocks that an SM holds
     floats = 2 * sms * 48 * (32 * -(-head_dim // 32) + 2)
     counters = max(1, num_seqs) * num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
-    return KV4Scratch(num_seqs, (num_heads, num_kv_heads, head_dim), sms, torch.empty(floats, dtype=torch.float32, device=device),
-                      torch.zeros(counters, dtype=torch.int32, device=device))
-
-
-def _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim, window):
-    """(type code, row strides of q and out, pages, page size, pages of a block table's row); `num_seqs` None: one per row of q."""
-    pages, page = _kv4_cache(op, cache, num_heads, num_kv_heads, head_dim)
-    code = _code(q, op)
-    q_stride = _kv4_rows(op, "q", q, None, num_heads * head_dim, q.dtype)
-    rows = q.shape[0]
-    out_stride = _kv4_rows(op, "out", out, rows, num_heads * head_dim, q.dtype)
-    shape = block_tables.shape
-    if block_tables.dtype is not torch.int32 or len(shape) != 2 or not block_tables.is_contiguous() or shape[1] < 1:
-        raise ShapeError(op, "block_tables must be contiguous int32 [S, max_pages]")
-    if shape[0] < (rows if num_seqs is None else num_seqs):
-        raise ShapeError(op, f"block_tables has {shape[0]} rows for {rows if num_seqs is None else num_seqs} requests")
-    if window < 0:
-        raise ShapeError(op, f"window {window} is negative")
-    return code, q_stride, out_stride, pages, page, shape[1]
+    return KV4Scratch((int(num_seqs), int(num_heads), int(num_kv_heads), int(head_dim)), sms,
+                      torch.empty(floats, dtype=torch.float32, device=device), torch.zeros(counters, dtype=torch.int32, device=device),
+                      _scratch_for(torch.device(device)).err)
 
 
 @_timed
@@ -2390,29 +2333,9 @@ def attn_decode_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     which becomes 0). q, out [S, H*hd]; `window`: a row sees itself and the window - 1 tokens before it (0: every earlier token).
     `scratch`: `kv4_scratch` for at least so many requests. A row whose page number lies outside the pool, or that sees a key or value
     kept as NaN, becomes NaN."""
-    op = "attn_decode_kv4"
-    partials, arrived = scratch.partials, scratch.arrived
-    dev = _kv4_device(op, q, out, cache, block_tables, positions, partials)
-    code, q_stride, out_stride, pages, page, max_pages = _kv4_attn_checks(op, q, out, cache, block_tables, None, num_heads, num_kv_heads, head_dim,
-                                                                          window)
-    S = q.shape[0]
-    _int32_vec(positions, S, op, "positions")
-    if scratch.sizes != (num_heads, num_kv_heads, head_dim) or S > scratch.num_seqs:
-        raise ShapeError(op, f"the scratch was made for {scratch.num_seqs} requests of {scratch.sizes}, not for {S} of "
-                             f"{(num_heads, num_kv_heads, head_dim)} (heads, kv heads, head size)")
-    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
-    if code == 1 and q_stride % 8 == 0 and q_ptr % 16 == 0 and out_stride % 2 == 0 and out_ptr % 4 == 0:
-        _check(_fn("kv4_decode", "vob_kv4_decode", _KV4_DECODE)(
-            q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, positions.data_ptr(), S, num_heads,
-            num_kv_heads, head_dim, page, scale, window, partials.data_ptr(), scratch.floats, arrived.data_ptr(), scratch.counters, scratch.sms,
-            _scratch_for(q.device).err.data_ptr(), _raw_stream(dev)), op, 1 if S else 0)
-        return
-    # 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address
-    splits = max(1, min(32, 2 * scratch.sms // max(1, S * num_kv_heads * -(-(num_heads // num_kv_heads) // 16))))
-    _check(_fn("kv4", "vob_kv4_attend", _KV4_ATTEND)(
-        q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, positions.data_ptr(), None, None, S, 1,
-        num_heads, num_kv_heads, head_dim, page, scale, window, code, splits, partials.data_ptr(), arrived.data_ptr(), _raw_stream(dev)),
-        op, 1 if S else 0)
+    n = _kv4_native or _kv4()
+    _kv4_done(n.decode(n.decode_entry, n.attend_entry, q, out, cache, block_tables, positions, num_heads, num_kv_heads, head_dim, scale, window,
+                       scratch.partials, scratch.arrived, scratch.made_for, scratch.sms, scratch.err_ptr), "attn_decode_kv4")
 
 
 @_timed
@@ -2423,26 +2346,9 @@ def attn_prefill_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, bl
     [T, H*hd]; seq_starts int32 [S+1] (first row of each request), context_lens int32 [S] (tokens cached before the step), max_new = the
     longest portion (a request's rows beyond it are not computed). `window` and what becomes NaN: as `attn_decode_kv4`. Rows that
     belong to no request are left as they are."""
-    op = "attn_prefill_kv4"
-    dev = _kv4_device(op, q, out, cache, block_tables, seq_starts, context_lens)
-    code, q_stride, out_stride, pages, page, max_pages = _kv4_attn_checks(op, q, out, cache, block_tables, num_seqs, num_heads, num_kv_heads, head_dim,
-                                                                          window)
-    _int32_vec(seq_starts, num_seqs + 1, op, "seq_starts")
-    _int32_vec(context_lens, num_seqs, op, "context_lens")
-    launches = 1 if num_seqs > 0 and max_new > 0 else 0
-    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
-    if (code == 1 and head_dim <= 128 and num_heads // num_kv_heads <= 128 and scale > 0 and q_stride % 8 == 0 and q_ptr % 16 == 0
-            and out_stride % 8 == 0 and out_ptr % 16 == 0):
-        _check(_fn("kv4_prefill", "vob_kv4_prefill", _KV4_PREFILL)(
-            q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, seq_starts.data_ptr(),
-            context_lens.data_ptr(), num_seqs, max_new, num_heads, num_kv_heads, head_dim, page, scale, window,
-            _scratch_for(q.device).err.data_ptr(), _raw_stream(dev)), op, launches)
-        return
-    # 32-bit arithmetic: the float32 engine, larger heads, and rows that the tensor-core kernel cannot address
-    _check(_fn("kv4", "vob_kv4_attend", _KV4_ATTEND)(
-        q_ptr, q_stride, out_ptr, out_stride, cache.data_ptr(), pages, block_tables.data_ptr(), max_pages, None, seq_starts.data_ptr(),
-        context_lens.data_ptr(), num_seqs, max_new, num_heads, num_kv_heads, head_dim, page, scale, window, code, 1, None, None, _raw_stream(dev)),
-        op, launches)
+    n = _kv4_native or _kv4()
+    _kv4_done(n.prefill(n.prefill_entry, n.attend_entry, q, out, cache, block_tables, seq_starts, context_lens, num_seqs, max_new, num_heads, num_kv_heads,
+                        head_dim, scale, window, _scratch_for(q.device).err.data_ptr()), "attn_prefill_kv4")
 
 
 # ------------------------------------------------------------------------------------ sampling
