@@ -314,17 +314,9 @@ kv4_read_kernel(const unsigned char* __restrict__ cache, long long num_slots, co
 }
 
 // ---------------------------------------------------------------------------------------------
-// Attention in 32-bit arithmetic, any head size up to 256 and any number of heads per kv head: the float32 engine's kernel, and the one
-// for portions of head sizes that the tensor-core kernel does not take.
-//
-// One block: ROWS rows (token, head of the group) of one request and kv head, over KEYS keys at a time: codes become numbers in
-// shared memory once per tile, each of 256 threads takes 4 rows x 1 key of the scores and 4 rows x DP / 64 numbers of the sums, the maximum
-// and the sum of a row run along in shared memory. `splits` blocks share a request's keys (single tokens); the last one to arrive adds their
-// partial results in the order of the keys, so the result does not depend on who that is.
-// Bound: the FMA pipe's operands in shared memory.
+// Attention in 32-bit arithmetic, any head size up to 256 and any number of heads per kv head: the float32 engine's kernels, and those for rows
+// and head sizes that the tensor-core kernels do not take. First single tokens, then portions.
 // ---------------------------------------------------------------------------------------------
-constexpr int ROWS = 16, KEYS = 64, FLEX_THREADS = 256;
-
 struct Batch {
     const int* positions;        // single tokens: row s is request s at this position (-1: a padding row). Otherwise null
     const int* seq_starts;
@@ -334,6 +326,199 @@ struct Batch {
     float scale;
 };
 
+// Eight codes as numbers: a code in the low bits of 2^23 is 2^23 + n.
+__device__ __forceinline__ float code_number(uint32_t w, int i) { return __uint_as_float((w >> (4 * i) & 15u) | 0x4b000000u) - 8388608.f; }
+
+// Single tokens. A block has 4 heads of one request and kv head, and `splits` blocks share the request's keys; each of its warps takes 32 keys at a time, by
+// itself: a lane a key for the scores, sum(q n) s + m sum(q) on the codes as they come from the cache, then two numbers a lane (NB times 64 numbers) for the
+// sums, the codes of the values going through shared memory. The warps' results meet at the end, the blocks' in the block that arrives last, in the
+// order of the keys. Bound: instructions (some 16 per key and 32 lanes for the scores, as many for the sums, at 4 heads of 64).
+constexpr int SINGLE_ROWS = 4, SINGLE_WARPS = 4;
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(32 * SINGLE_WARPS, 4)
+kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const unsigned char* __restrict__ cache, Batch b,
+                  int splits, float* __restrict__ partials, int* __restrict__ arrived) {
+    constexpr int R = SINGLE_ROWS, W = SINGLE_WARPS, DP = 64 * NB, TILE = 32 * W;
+    __shared__ __align__(16) float sQ[R][DP];
+    __shared__ float sum_q[R], sM[W][R], sL[W][R];
+    __shared__ __align__(16) float4 sP[W][32];
+    __shared__ __align__(16) unsigned char sV[W][32][32 * NB];
+    __shared__ float sO[W][R][DP];
+    __shared__ int is_last;
+    pdl_launch_dependents();
+    pdl_wait(35);
+    const int seq = blockIdx.z, split = blockIdx.x, group = b.H / b.G, hd = b.hd;
+    const int row_tiles = (group + R - 1) / R, g = blockIdx.y / row_tiles, head0 = g * group + blockIdx.y % row_tiles * R;
+    const int heads = min(R, (g + 1) * group - head0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hi = b.positions[seq] + 1, lo = b.window ? max(0, hi - b.window) : 0;
+    if (hi <= 0) {                                          // a padding row sees nothing
+        if (split == 0)
+            for (int i = threadIdx.x; i < heads * hd; i += 32 * W) st_f(out + (size_t)seq * out_stride + (size_t)head0 * hd + i, 0.f);
+        return;
+    }
+    const int t_lo = lo / TILE, t_hi = (hi + TILE - 1) / TILE, share = (t_hi - t_lo + splits - 1) / splits;
+    const int used = (t_hi - t_lo + share - 1) / share, t0 = t_lo + split * share, t1 = min(t_hi, t0 + share);
+    if (t0 >= t1) return;
+    for (int i = threadIdx.x; i < R * DP; i += 32 * W) {
+        const int r = i / DP, d = i % DP;
+        sQ[r][d] = r < heads && d < hd ? ld_f(q + (size_t)seq * q_stride + (size_t)(head0 + r) * hd + d) * b.scale : 0.f;
+    }
+    __syncthreads();
+    if (warp < R) {
+        float v = 0.f;
+        for (int d = lane; d < DP; d += 32) v += sQ[warp][d];
+        v = warp_sum(v);
+        if (lane == 0) sum_q[warp] = v;
+    }
+    __syncthreads();
+    const int C = chunks(hd), width = token_bytes(hd);
+    const int* bt = b.block_tables + (size_t)seq * b.max_pages;
+    float m[R], l[R], base[R], acc[R][2 * NB];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = base[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) acc[r][i] = 0.f;
+    }
+    for (int tile = t0; tile < t1; ++tile) {
+        const int key = tile * TILE + warp * 32 + lane;
+        const bool in = key >= lo && key < hi;
+        if (!__any_sync(0xffffffffu, in)) continue;
+        float2 ks = make_float2(0.f, 0.f), vs = ks;
+        const unsigned char* grp = nullptr;
+        if (in) {
+            const int pi = key / b.page_size, off = key - pi * b.page_size;
+            const int page = pi < b.max_pages ? bt[pi] : -1;
+            if (page >= 0 && page < b.num_pages) {
+                grp = cache + group_at(page, g, off, b.G, b.page_size, width) + (off & 7) * 16;
+                attend_scales(*reinterpret_cast<const uint2*>(grp + 256 * C - (off & 7) * 8), ks, vs);
+            } else {
+                ks = make_float2(NAN, NAN);                 // a page outside the pool: the rows that see it become NaN
+            }
+        }
+        float s[R] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < C; ++c) {
+            uint4 kn = make_uint4(0, 0, 0, 0), vn = kn;
+            if (grp) {
+                kn = *reinterpret_cast<const uint4*>(grp + c * 128);
+                vn = *reinterpret_cast<const uint4*>(grp + (C + c) * 128);
+            }
+            *reinterpret_cast<uint4*>(&sV[warp][lane][16 * c]) = vn;
+            const uint32_t w[4] = {kn.x, kn.y, kn.z, kn.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float n0 = code_number(w[u], 4 * h), n1 = code_number(w[u], 4 * h + 1), n2 = code_number(w[u], 4 * h + 2), n3 = code_number(w[u], 4 * h + 3);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float4 qx = *reinterpret_cast<const float4*>(&sQ[r][32 * c + 8 * u + 4 * h]);
+                        s[r] = fmaf(n3, qx.w, fmaf(n2, qx.z, fmaf(n1, qx.y, fmaf(n0, qx.x, s[r]))));
+                    }
+                }
+        }
+        float p[R], scale_o[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s[r] = in ? fmaf(s[r], ks.x, ks.y * sum_q[r]) : -INFINITY;
+            const float to = fmaxf(m[r], warp_max(s[r])), use = to == -INFINITY ? 0.f : to;
+            scale_o[r] = m[r] == -INFINITY ? 0.f : expf(m[r] - use);
+            m[r] = to;
+            p[r] = expf(s[r] - use);
+            l[r] = fmaf(l[r], scale_o[r], p[r]);
+            base[r] = fmaf(base[r], scale_o[r], p[r] * vs.y);
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i) acc[r][i] *= scale_o[r];
+        }
+        sP[warp][lane] = make_float4(p[0] * vs.x, p[1] * vs.x, p[2] * vs.x, p[3] * vs.x);
+        __syncwarp();
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) {
+            const float4 w = sP[warp][k];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t two = sV[warp][k][lane + 32 * i];
+                const float n0 = code_number(two, 0), n1 = code_number(two, 1);
+                acc[0][2 * i] = fmaf(w.x, n0, acc[0][2 * i]);
+                acc[0][2 * i + 1] = fmaf(w.x, n1, acc[0][2 * i + 1]);
+                acc[1][2 * i] = fmaf(w.y, n0, acc[1][2 * i]);
+                acc[1][2 * i + 1] = fmaf(w.y, n1, acc[1][2 * i + 1]);
+                acc[2][2 * i] = fmaf(w.z, n0, acc[2][2 * i]);
+                acc[2][2 * i + 1] = fmaf(w.z, n1, acc[2][2 * i + 1]);
+                acc[3][2 * i] = fmaf(w.w, n0, acc[3][2 * i]);
+                acc[3][2 * i + 1] = fmaf(w.w, n1, acc[3][2 * i + 1]);
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] = warp_sum(l[r]);
+        base[r] = warp_sum(base[r]);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {                       // byte lane + 32 i of a vector: numbers 2 lane + 64 i and the next
+            sO[warp][r][2 * lane + 64 * i] = acc[r][2 * i] + base[r];
+            sO[warp][r][2 * lane + 64 * i + 1] = acc[r][2 * i + 1] + base[r];
+        }
+        if (lane == 0) { sM[warp][r] = m[r]; sL[warp][r] = l[r]; }
+    }
+    __syncthreads();
+    // a part without keys has nothing to weigh (its sums are 0); one whose keys all gave NaN has no maximum either, and stays NaN
+    auto weight = [](float mine, float all) { return mine == -INFINITY ? 1.f : expf(mine - all); };
+    const size_t unit = (size_t)seq * gridDim.y + blockIdx.y, each = (size_t)R * (hd + 2);
+    float* mine = partials + (unit * splits + split) * each;
+    for (int i = threadIdx.x; i < heads * hd; i += 32 * W) {
+        const int r = i / hd, d = i - r * hd;
+        float all = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) all = fmaxf(all, sM[w][r]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = weight(sM[w][r], all);
+            sum = fmaf(f, sL[w][r], sum);
+            o = fmaf(f, sO[w][r][d], o);
+        }
+        if (used == 1) {
+            st_f(out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d, o / sum);
+        } else {
+            mine[i] = o;
+            if (d == 0) { mine[R * hd + r] = all; mine[R * hd + R + r] = sum; }
+        }
+    }
+    if (used == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        is_last = atomicAdd(arrived + unit, 1) == used - 1;
+        if (is_last) arrived[unit] = 0;                     // as it was found, for the next launch
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    const float* parts = partials + unit * splits * each;
+    for (int i = threadIdx.x; i < heads * hd; i += 32 * W) {
+        const int r = i / hd, d = i - r * hd;
+        float all = -INFINITY, sum = 0.f, o = 0.f;
+        for (int c = 0; c < used; ++c) all = fmaxf(all, __ldcg(parts + c * each + R * hd + r));
+#pragma unroll 4
+        for (int c = 0; c < used; ++c) {
+            const float f = weight(__ldcg(parts + c * each + R * hd + r), all);
+            sum = fmaf(f, __ldcg(parts + c * each + R * hd + R + r), sum);
+            o = fmaf(f, __ldcg(parts + c * each + i), o);
+        }
+        st_f(out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d, o / sum);
+    }
+}
+
+// Portions. One block: ROWS rows (token, head of the group) of one request and kv head, over KEYS keys at a time: codes become numbers in
+// shared memory once per tile, each of 256 threads takes 4 rows x 1 key of the scores and 4 rows x DP / 64 numbers of the sums, the maximum
+// and the sum of a row run along in shared memory.
+// Bound: the FMA pipe's operands in shared memory.
+constexpr int ROWS = 16, KEYS = 64, FLEX_THREADS = 256;
+
 template <int DP> constexpr size_t flex_smem() {
     return sizeof(float) * ((size_t)KEYS * (DP + 4) + (size_t)KEYS * DP + ROWS * DP + KEYS * ROWS + 3 * ROWS);
 }
@@ -341,7 +526,7 @@ template <int DP> constexpr size_t flex_smem() {
 template <typename T, int DP>
 __global__ void __launch_bounds__(FLEX_THREADS)
 kv4_attend_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const unsigned char* __restrict__ cache,
-                  Batch b, int splits, float* __restrict__ partials, int* __restrict__ arrived) {
+                  Batch b) {
     extern __shared__ float4 smem4[];
     float* sK = reinterpret_cast<float*>(smem4);           // [KEYS][DP + 4]
     float* sV = sK + KEYS * (DP + 4);                      // [KEYS][DP]
@@ -350,35 +535,18 @@ kv4_attend_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
     float* sM = sP + KEYS * ROWS;                          // [ROWS] running maximum
     float* sL = sM + ROWS;                                 // [ROWS] running sum
     float* sA = sL + ROWS;                                 // [ROWS] factor of this tile for what came before
-    __shared__ int is_last;
     pdl_launch_dependents();
     pdl_wait(32);
-    const int seq = blockIdx.z / splits, split = blockIdx.z % splits, g = blockIdx.y;
+    const int seq = blockIdx.z, g = blockIdx.y;
     const int group = b.H / b.G, hd = b.hd, tid = threadIdx.x;
-    const int row0 = b.positions ? seq : b.seq_starts[seq];
-    const int tokens = b.positions ? 1 : b.seq_starts[seq + 1] - row0;
-    const int ctx = b.positions ? b.positions[seq] : b.context_lens[seq];
+    const int row0 = b.seq_starts[seq], tokens = b.seq_starts[seq + 1] - row0, ctx = b.context_lens[seq];
     const int total = tokens * group, tile0 = blockIdx.x * ROWS;
     if (tile0 >= total) return;
     const int nrows = min(ROWS, total - tile0);
     const int last_tok = (tile0 + nrows - 1) / group, first_tok = tile0 / group;
     const int hi = ctx + last_tok + 1;                                                    // keys any row sees: [lo, hi)
     const int lo = b.window ? max(0, ctx + first_tok - b.window + 1) : 0;
-    if (hi <= 0) {                                                                        // a padding row sees nothing
-        if (split == 0)
-            for (int i = tid; i < nrows * hd; i += FLEX_THREADS) {
-                const int r = tile0 + i / hd;
-                st_f(out + (size_t)(row0 + r / group) * out_stride + (size_t)(g * group + r % group) * hd + i % hd, 0.f);
-            }
-        return;
-    }
-    // this block's tiles of keys
-    const int t_lo = lo / KEYS, t_hi = (hi + KEYS - 1) / KEYS;
-    const int share = (t_hi - t_lo + splits - 1) / splits;
-    const int t0 = t_lo + split * share, t1 = min(t_hi, t0 + share);
-    const int used = (t_hi - t_lo + share - 1) / share;                                  // splits that have keys
-    if (t0 >= t1) return;
-
+    const int t0 = lo / KEYS, t1 = (hi + KEYS - 1) / KEYS;                               // tiles of keys
     for (int i = tid; i < ROWS * DP; i += FLEX_THREADS) {
         const int r = i / DP, d = i % DP, rr = tile0 + r;
         sQ[i] = (r < nrows && d < hd) ? ld_f(q + (size_t)(row0 + rr / group) * q_stride + (size_t)(g * group + rr % group) * hd + d) * b.scale : 0.f;
@@ -485,51 +653,6 @@ kv4_attend_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
             }
         }
     }
-    if (used > 1) {
-        // partial of this split: [ROWS][hd] sums, then maxima and sums of the rows
-        const size_t unit = (size_t)(seq * b.G + g) * gridDim.x + blockIdx.x;
-        const size_t each = (size_t)ROWS * (hd + 2);
-        float* mine = partials + (unit * splits + split) * each;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-                if (key + 64 * d < hd) mine[(rg + r) * hd + key + 64 * d] = acc[r][d];
-        if (tid < ROWS) { mine[ROWS * hd + tid] = sM[tid]; mine[ROWS * hd + ROWS + tid] = sL[tid]; }
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            is_last = atomicAdd(arrived + unit, 1) == used - 1;
-            if (is_last) arrived[unit] = 0;                // as it was found, for the next launch
-        }
-        __syncthreads();
-        if (!is_last) return;
-        __threadfence();
-        const float* all = partials + unit * splits * each;
-        if (tid < ROWS) {
-            float m = -INFINITY;
-            for (int s = 0; s < used; ++s) m = fmaxf(m, __ldcg(all + s * each + ROWS * hd + tid));
-            sM[tid] = m;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float l = 0.f;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) acc[r][d] = 0.f;
-            const float m = sM[rg + r];
-            for (int s = 0; s < used; ++s) {
-                const float* part = all + s * each;
-                const float ms = __ldcg(part + ROWS * hd + rg + r);
-                const float a = ms == -INFINITY ? 0.f : expf(ms - m);
-                l += a * __ldcg(part + ROWS * hd + ROWS + rg + r);
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    if (key + 64 * d < hd) acc[r][d] = fmaf(a, __ldcg(part + (rg + r) * hd + key + 64 * d), acc[r][d]);
-            }
-            if (key == 0) sL[rg + r] = l;
-        }
-    }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -546,6 +669,12 @@ kv4_attend_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
 template <typename T, int DP>
 int launch_attend(const void* q, long long q_stride, void* out, long long out_stride, const unsigned char* cache, const Batch& b, int S,
                   int max_new, int splits, float* partials, int* arrived, cudaStream_t stream) {
+    if (b.positions) {
+        const long long units = (long long)b.G * ((b.H / b.G + SINGLE_ROWS - 1) / SINGLE_ROWS);
+        if (units > 65535 || S > 65535) return VOB_ERR_UNSUPPORTED;
+        return vob_launch(kv4_single_kernel<T, DP / 64>, dim3(splits, (unsigned)units, S), dim3(32 * SINGLE_WARPS), 0, stream, (const T*)q, q_stride,
+                          (T*)out, out_stride, cache, b, splits, partials, arrived);
+    }
     // once per device that the process uses: the attribute belongs to the current one
     static size_t done[64] = {};
     int dev = 0;
@@ -557,9 +686,9 @@ int launch_attend(const void* q, long long q_stride, void* out, long long out_st
         if (dev < 64) done[dev] = 1;
     }
     const long long tiles = ((long long)max_new * (b.H / b.G) + ROWS - 1) / ROWS;
-    if (tiles > 0x7fffffffLL || b.G > 65535 || (long long)S * splits > 65535) return VOB_ERR_UNSUPPORTED;
-    return vob_launch(kv4_attend_kernel<T, DP>, dim3((unsigned)tiles, b.G, S * splits), dim3(FLEX_THREADS), flex_smem<DP>(), stream,
-                      (const T*)q, q_stride, (T*)out, out_stride, cache, b, splits, partials, arrived);
+    if (tiles > 0x7fffffffLL || b.G > 65535 || S > 65535) return VOB_ERR_UNSUPPORTED;
+    return vob_launch(kv4_attend_kernel<T, DP>, dim3((unsigned)tiles, b.G, S), dim3(FLEX_THREADS), flex_smem<DP>(), stream,
+                      (const T*)q, q_stride, (T*)out, out_stride, cache, b);
 }
 
 bool sizes_ok(int H, int G, int hd, int page_size) {
@@ -607,14 +736,20 @@ VOB_EXPORT int vob_kv4_read(const void* cache, long long num_pages, const int* s
 }
 
 // Attention in 32-bit arithmetic. Single tokens: `positions` int32 [S] (row s of q is request s); otherwise seq_starts int32 [S + 1] and
-// context_lens int32 [S]. `partials` (splits > 1): S * G * row tiles * splits * 16 * (hd + 2) floats; `arrived`: S * G * row tiles zeros.
+// context_lens int32 [S]. `splits` blocks share a single token's keys, meeting in `partials` (S * G * ceil(H / G / 4) * splits * 4 * (hd + 2) floats; as
+// many as `partial_floats` lets there be) and `arrived` (S * G * ceil(H / G / 4) zeros).
 VOB_EXPORT int vob_kv4_attend(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, long long num_pages,
                               const int* block_tables, int max_pages, const int* positions, const int* seq_starts, const int* context_lens,
                               int S, int max_new, int H, int G, int hd, int page_size, float scale, int window, int code, int splits,
-                              float* partials, int* arrived, cudaStream_t stream) {
+                              float* partials, long long partial_floats, int* arrived, long long counters, cudaStream_t stream) {
     if (S <= 0 || max_new <= 0) return 0;
     if (!sizes_ok(H, G, hd, page_size) || num_pages <= 0 || num_pages > 0x7fffffffLL || splits <= 0 || window < 0) return VOB_ERR_BAD_ARG;
-    if (splits > 1 && (!partials || !arrived || !positions)) return VOB_ERR_BAD_ARG;
+    if (splits > 1) {
+        if (!partials || !arrived || !positions) return VOB_ERR_BAD_ARG;
+        const long long units = (long long)S * G * ((H / G + SINGLE_ROWS - 1) / SINGLE_ROWS);
+        if (counters < units) return VOB_ERR_BAD_ARG;
+        splits = (int)max(1LL, min((long long)splits, partial_floats / (units * SINGLE_ROWS * (hd + 2))));
+    }
     if (!positions && (!seq_starts || !context_lens)) return VOB_ERR_BAD_ARG;
     Batch b = {positions, seq_starts, context_lens, block_tables, max_pages, (int)num_pages, page_size, window, H, G, hd, scale};
     const unsigned char* c = (const unsigned char*)cache;

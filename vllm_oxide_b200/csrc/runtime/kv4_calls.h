@@ -160,7 +160,7 @@ typedef int (*AppendFn)(const void*, long long, void*, long long, const void*, l
                         long long, int, int, int, int, int, int, void*);
 typedef int (*ReadFn)(const void*, long long, const int*, void*, long long, void*, long long, int, int, int, int, int, void*);
 typedef int (*AttendFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, const int*, const int*, int, int, int,
-                        int, int, int, float, int, int, int, float*, int*, void*);
+                        int, int, int, float, int, int, int, float*, long long, int*, long long, void*);
 typedef int (*DecodeFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, int, int, int, int, int, float, int,
                         float*, long long, int*, long long, int, int*, void*);
 typedef int (*PrefillFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, const int*, int, int, int, int, int,
@@ -263,13 +263,13 @@ inline PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t count) {
         return PyLong_FromLong(((DecodeFn)entry)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
                                                  (int*)pos.ptr, (int)S, (int)H, (int)G, (int)hd, (int)cache.size[2], (float)scale, (int)window,
                                                  (float*)partials.ptr, partials.size[0], (int*)arrived.ptr, arrived.size[0], (int)sms, (int*)err, stream));
-    // 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address
-    const long long tiles = (H / G + 15) / 16, blocks = S * G * tiles;
-    long long splits = 2 * sms / blocks;
-    splits = splits < 1 ? 1 : splits > 32 ? 32 : splits;
+    // 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address. Blocks of 4 heads, eight an SM
+    const long long blocks = S * G * ((H / G + 3) / 4);
+    long long splits = 8 * sms / blocks;
+    splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     return PyLong_FromLong(((AttendFn)general)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
                                                (int*)pos.ptr, nullptr, nullptr, (int)S, 1, (int)H, (int)G, (int)hd, (int)cache.size[2], (float)scale,
-                                               (int)window, q.code(), (int)splits, (float*)partials.ptr, (int*)arrived.ptr, stream));
+                                               (int)window, q.code(), (int)splits, (float*)partials.ptr, partials.size[0], (int*)arrived.ptr, arrived.size[0], stream));
 }
 
 // (entry, entry in 32-bit arithmetic, q, out, cache, block_tables, seq_starts, context_lens, requests, longest portion, heads, kv heads, head size, scale,
@@ -299,7 +299,7 @@ inline PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t count) {
     // 32-bit arithmetic: the float32 engine, larger heads, and rows that the tensor-core kernel cannot address
     return PyLong_FromLong(((AttendFn)general)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
                                                nullptr, (int*)starts.ptr, (int*)contexts.ptr, (int)S, (int)longest, (int)H, (int)G, (int)hd,
-                                               (int)cache.size[2], (float)scale, (int)window, q.code(), 1, nullptr, nullptr, stream));
+                                               (int)cache.size[2], (float)scale, (int)window, q.code(), 1, nullptr, 0, nullptr, 0, stream));
 }
 
 // (ShapeError, KernelError, float32, bfloat16, uint8, int32, get_device, raw_stream): what the calls need to know of Python, once.

@@ -2320,7 +2320,7 @@ def kv4_scratch(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
     sms = torch.cuda.get_device_properties(device).multi_processor_count
     # two partial results per block; at most 48 heads in the blocks that an SM holds
     floats = 2 * sms * 48 * (32 * -(-head_dim // 32) + 2)
-    counters = max(1, num_seqs) * num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
+    counters = max(1, num_seqs) * num_kv_heads * -(-(num_heads // num_kv_heads) // 4)
     return KV4Scratch((int(num_seqs), int(num_heads), int(num_kv_heads), int(head_dim)), sms,
                       torch.empty(floats, dtype=torch.float32, device=device), torch.zeros(counters, dtype=torch.int32, device=device),
                       _scratch_for(torch.device(device)).err)
