@@ -4,18 +4,20 @@
 //   score_j = scale (ks_j (q . n_j) + km_j sum(q)),     p_j = 2^(score_j log2 e - M),
 //   out = (sum_j (p_j vs_j) w_j + sum_j p_j vm_j) / sum_j p_j.
 // Both products run on the codes themselves, by mma.sync in float16 with float32 sums; scales and minima come in once per
-// (head, key). A code needs no conversion: four bits alone in the low mantissa of a float16 are the number n 2^-24 (a subnormal, exact), four
-// bits one place higher 16 n 2^-24. So a 32-bit word of eight codes becomes four operand registers in five instructions (a shift by 8 and
-// four masks); the factors 16 are taken out of q (keys) and of the results (values).
-//   * q enters as float16: a bfloat16 has 8 bits and fits, times a power of two that brings the unit's largest number to 2^14 .. 2^15
-//     (numbers 2^28 below the largest start to lose bits).
+// (head, key). A code needs no conversion: the low bits of a float16's mantissa alone are a whole number times 2^-24 (a subnormal, exact), so a byte
+// of two codes is n0 + 16 n1, and its low half n0. A 32-bit word of eight codes becomes four operand registers in four instructions (the two bytes
+// of each half by a mask and a byte permutation, two masks more): n0 with the weight q0 - q1 / 16 and n0 + 16 n1 with q1 / 16 for the keys, and the
+// values' sums of n0 and of n0 + 16 n1 are told apart at the end.
+//   * q enters as float16 times a power of two that brings the unit's largest number to 2^14 .. 2^15 (numbers 2^28 below the largest start to
+//     lose bits): q1 / 16 is exact, q0 - q1 / 16 is rounded to 11 bits, 2^-12 of it.
 //   * p_j vs_j is rounded to float16, 11 bits (2^-12 of it on average less than bfloat16's 2^-9, which would be seen: the codes' sum is large
 //     against the result, which is the difference of it and the minima's). M is chosen from score_j log2 e + log2 vs_j, so that these products use
 //     float16's range from the top: at most 2^15, set to 2^4 when M moves. M moves only when a product would pass 2^15 (a vote per 32 keys;
 //     no reductions between lanes otherwise), and the sums so far are scaled once then.
 //   * sums of p_j, of p_j vm_j and of the products are float32.
 // Operands: S^T = N Q^T (A = 16 keys x 16 numbers straight from ldmatrix, B = Q^T, 8 heads) and O^T = W^T P^T (A = 16 numbers x 16 keys from
-// ldmatrix.trans, B = P^T by movmatrix of the scores' registers): eight heads a product fill an instruction that would be half empty with heads as rows.
+// ldmatrix.trans, B = P^T by movmatrix of the scores' registers): eight heads a product fill an instruction that would be half empty with heads as rows. Up to
+// four heads (SMALL), the lanes that would have heads 4 to 7 take the second 16 keys' scores of heads 0 to 3.
 //
 // Work. The keys of all (request, kv head, heads) units, in rounds of 128, lie one behind the other; every block takes an equal share of
 // consecutive rounds, whatever the requests' lengths. In a round each of 4 warps has 32 keys, which it fetches itself (bulk copies of
@@ -38,7 +40,8 @@ constexpr float P_LIMIT = 32768.f, P_TOP = 4.f;
 
 // NC chunks of 32 numbers, NT times 8 heads. Blocks per SM and stages of a warp's ring: as many bytes in flight as registers and
 // shared memory allow (4 blocks of 4 warps at head sizes up to 128).
-template <int NC, int NT> struct Sizes {
+template <int NC, int NT, bool SMALL> struct Sizes {
+    static constexpr int KEYS = SMALL ? 2 : 4;                    // keys of a lane in a step
     static constexpr int SUB = 256 * NC + 64;                     // bytes of eight keys and values
     static constexpr int TILE = NC <= 2 ? 64 : 32;                // keys of a stage of a warp's ring: one or two steps
     static constexpr int ROUND = TILE * WARPS;                    // keys that a block takes at a time
@@ -90,6 +93,14 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
 }
+// Of every word its codes 0 and 4 (half 1: 2 and 6) as they are, and with the next ones, times 16, added.
+__device__ __forceinline__ void codes(const uint32_t (&w)[4], int half, uint32_t (&low)[4], uint32_t (&both)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        both[i] = half ? __byte_perm(w[i], 0, 0x4341) : w[i] & 0x00ff00ffu;
+        low[i] = both[i] & 0x000f000fu;
+    }
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -111,10 +122,12 @@ struct Place {
     int s, gh, k;
 };
 
-template <int NC, int NT>
-__global__ void __launch_bounds__(THREADS, Sizes<NC, NT>::BLOCKS)
+template <int NC, int NT, bool SMALL>
+__global__ void __launch_bounds__(THREADS, Sizes<NC, NT, SMALL>::BLOCKS)
 kv4_decode_kernel(const Args a) {
-    using Z = Sizes<NC, NT>;
+    using Z = Sizes<NC, NT, SMALL>;
+    static_assert(!SMALL || NT == 1, "four heads at most");
+    constexpr int KEYS = Z::KEYS, MERGED = SMALL ? 4 : 8;                          // heads that a pass of the merge writes
     using Span = SpanOf<Z::ROUND>;
     constexpr int TILE = Z::TILE, ROUND = Z::ROUND;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -258,7 +271,8 @@ kv4_decode_kernel(const Args a) {
         const int kvh = at.gh / a.head_tiles, head0 = kvh * group + (at.gh % a.head_tiles) * Z::HEADS;
         const int heads = min(Z::HEADS, kvh * group + group - head0);
         const int k_end = min(span.count, at.k + (x1 - x));
-        // Q^T as the B operand: lane (head g8, c4) holds numbers 32c + 8 c4 + {0,4}, {1,5} / 16, {2,6}, {3,7} / 16 of each chunk
+        // Q^T as the B operand: lane (head g8, c4) holds of numbers 32c + 8 c4 + 0 .. 7 of each chunk {0,4} - {1,5} / 16, {1,5} / 16, {2,6} - {3,7} / 16,
+        // {3,7} / 16
         uint32_t qf[NT][NC][4];
         float qs[NT][2];
         float to_score;                                                             // scale log2 e 2^24 / (the power of two that q was given)
@@ -303,16 +317,16 @@ kv4_decode_kernel(const Args a) {
                     float f[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16) * up; f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * up; }
-                    qf[n][c][0] = pack_half2(f[0], f[4]);
+                    qf[n][c][0] = pack_half2(fmaf(f[1], -0.0625f, f[0]), fmaf(f[5], -0.0625f, f[4]));
                     qf[n][c][1] = pack_half2(f[1] * 0.0625f, f[5] * 0.0625f);
-                    qf[n][c][2] = pack_half2(f[2], f[6]);
+                    qf[n][c][2] = pack_half2(fmaf(f[3], -0.0625f, f[2]), fmaf(f[7], -0.0625f, f[6]));
                     qf[n][c][3] = pack_half2(f[3] * 0.0625f, f[7] * 0.0625f);
                 }
                 float t = sum[n] * a.scale_log2;
                 t += __shfl_xor_sync(0xffffffffu, t, 1);
                 t += __shfl_xor_sync(0xffffffffu, t, 2);
-                qs[n][0] = __shfl_sync(0xffffffffu, t, 8 * c4);                      // heads 2 c4 and 2 c4 + 1: the scores' columns
-                qs[n][1] = __shfl_sync(0xffffffffu, t, 8 * c4 + 4);
+                qs[n][0] = __shfl_sync(0xffffffffu, t, SMALL ? 8 * (c4 & 1) : 8 * c4);     // heads 2 c4 and 2 c4 + 1: the scores' columns
+                qs[n][1] = __shfl_sync(0xffffffffu, t, (SMALL ? 8 * (c4 & 1) : 8 * c4) + 4);
             }
         }
         float ref[NT][2], l[NT][2], base_v[NT][2], o[NT][NC][2][4];
@@ -361,39 +375,49 @@ kv4_decode_kernel(const Args a) {
             const uint32_t row_at = st_at + (lane >> 3) * Z::SUB + (lane & 7) * 16;   // matrix lane / 8 = eight keys
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                uint32_t w[4];
+                uint32_t w[4], low[4], both[4];
                 ldsm4(w, row_at + 128 * c);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int half = 0; half < 2; ++half) {
+                    codes(w, half, low, both);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        mma(s[t][n], w[2 * t] & 0x000f000fu, w[2 * t + 1] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x00f000f0u,
-                            qf[n][c][0], qf[n][c][1]);
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] >>= 8;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        mma(s[t][n], w[2 * t] & 0x000f000fu, w[2 * t + 1] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x00f000f0u,
-                            qf[n][c][2], qf[n][c][3]);
+                        for (int t = 0; t < 2; ++t)
+                            mma(s[t][n], low[2 * t], low[2 * t + 1], both[2 * t], both[2 * t + 1], qf[n][c][2 * half], qf[n][c][2 * half + 1]);
+                }
             }
-            // scales and minima of this lane's keys g8, g8 + 8, + 16, + 24
-            float2 ks[4], vs[4];
-            float vt[4];                                                             // the value's scale, as the reference takes it
-            const bool edge = first_key < span.lo || first_key + STEP > span.hi;
-            unsigned seen = 15u;
+            // the lane's scores: z[key][head] of its keys g8 + 8 key (SMALL: from key 16 on for the lanes that heads 4 to 7 would be for)
+            float z[NT][KEYS][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint2 w = *reinterpret_cast<const uint2*>(st + i * Z::SUB + 256 * NC + 8 * g8);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int key = 0; key < KEYS; ++key)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (SMALL) {
+                            const float other = __shfl_xor_sync(0xffffffffu, s[1][0][2 * key + h], 2);
+                            z[n][key][h] = c4 < 2 ? s[0][0][2 * key + h] : other;
+                        } else {
+                            z[n][key][h] = s[key >> 1][n][2 * (key & 1) + h];
+                        }
+                    }
+            const int first8 = SMALL ? 2 * (c4 >> 1) : 0;                            // the first of the groups of eight that its keys are in
+            float2 ks[KEYS], vs[KEYS];                                               // scales and minima
+            float vt[KEYS];                                                             // the value's scale, as the reference takes it
+            const bool edge = first_key < span.lo || first_key + STEP > span.hi;
+            unsigned seen = (1u << KEYS) - 1u;
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) {
+                const uint2 w = *reinterpret_cast<const uint2*>(st + (first8 + i) * Z::SUB + 256 * NC + 8 * g8);
                 ks[i] = scale_min(w.x);
                 vs[i] = scale_min(w.y);
                 ks[i].x *= to_score;
             }
             if (edge) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = first_key + 8 * i + g8;
+                for (int i = 0; i < KEYS; ++i) {
+                    const int j = first_key + 8 * (first8 + i) + g8;
                     if (j < span.lo || j >= span.hi) {                               // whatever lies there
                         seen &= ~(1u << i);
                         ks[i] = vs[i] = make_float2(0.f, 0.f);
@@ -402,52 +426,47 @@ kv4_decode_kernel(const Args a) {
             }
             // below 2^-40 a scale counts as that: p itself stays below 2^55, whatever the values of the keys with large scores
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vt[i] = fmaxf(vs[i].x, 9.094947e-13f);
-            float p[2][NT][4], most = 0.f;                                           // the largest p_j times scale
+            for (int i = 0; i < KEYS; ++i) vt[i] = fmaxf(vs[i].x, 9.094947e-13f);
+            float p[NT][KEYS][2], most = 0.f;                                           // the largest p_j times scale
             auto weigh = [&](int n) {
-                float e[4][2];
+                float e[KEYS][2];
 #pragma unroll
-                for (int key = 0; key < 4; ++key)
+                for (int key = 0; key < KEYS; ++key)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) e[key][h] = fmaf(ks[key].y, qs[n][h], -ref[n][h]);
                 if (edge) {
 #pragma unroll
-                    for (int key = 0; key < 4; ++key)
+                    for (int key = 0; key < KEYS; ++key)
                         if (!(seen >> key & 1)) e[key][0] = e[key][1] = -INFINITY;
                 }
 #pragma unroll
-                for (int key = 0; key < 4; ++key) {
+                for (int key = 0; key < KEYS; ++key) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float x = exp2_fast(fmaf(s[key >> 1][n][2 * (key & 1) + h], ks[key].x, e[key][h]));
-                        p[key >> 1][n][2 * (key & 1) + h] = x;
-                        e[key][h] = x;
-                    }
-                    most = fmaxf(most, fmaxf(e[key][0], e[key][1]) * vt[key]);       // (NaN is left out: it stays in p)
+                    for (int h = 0; h < 2; ++h) p[n][key][h] = exp2_fast(fmaf(z[n][key][h], ks[key].x, e[key][h]));
+                    most = fmaxf(most, fmaxf(p[n][key][0], p[n][key][1]) * vt[key]); // (NaN is left out: it stays in p)
                 }
             };
 #pragma unroll
             for (int n = 0; n < NT; ++n) weigh(n);
             if (__any_sync(0xffffffffu, most > P_LIMIT)) {
                 // a new reference: the largest score + log2 of its value's scale
-                float lg[4];
+                float lg[KEYS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lg[i] = log2f(vt[i]) - P_TOP;
+                for (int i = 0; i < KEYS; ++i) lg[i] = log2f(vt[i]) - P_TOP;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                    for (int key = 0; key < KEYS; ++key)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = 2 * t + (i >> 1);
-                            const float y = fmaf(s[t][n][i], ks[key].x, ks[key].y * qs[n][i & 1]) + lg[key];
-                            if (seen >> key & 1) top[i & 1] = fmaxf(top[i & 1], y);
+                        for (int h = 0; h < 2; ++h) {
+                            const float y = fmaf(z[n][key][h], ks[key].x, ks[key].y * qs[n][h]) + lg[key];
+                            if (seen >> key & 1) top[h] = fmaxf(top[h], y);
                         }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+                        for (int off = SMALL ? 2 : 4; off < 32; off <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
                         const float to = fmaxf(ref[n][i], top[i]);
                         const float f = ref[n][i] == -INFINITY ? 0.f : exp2_fast(ref[n][i] - to);
                         ref[n][i] = to;
@@ -465,30 +484,33 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int key = 0; key < KEYS; ++key) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = 2 * t + (i >> 1);
-                        l[n][i & 1] += p[t][n][i];
-                        base_v[n][i & 1] = fmaf(p[t][n][i], vs[key].y, base_v[n][i & 1]);
+                    for (int h = 0; h < 2; ++h) {
+                        l[n][h] += p[n][key][h];
+                        base_v[n][h] = fmaf(p[n][key][h], vs[key].y, base_v[n][h]);
                     }
-                    pb[n][t][0] = transpose8(pack_half2(p[t][n][0] * vs[2 * t].x, p[t][n][1] * vs[2 * t].x));
-                    pb[n][t][1] = transpose8(pack_half2(p[t][n][2] * vs[2 * t + 1].x, p[t][n][3] * vs[2 * t + 1].x));
+                    const uint32_t two = pack_half2(p[n][key][0] * vs[key].x, p[n][key][1] * vs[key].x);
+                    if constexpr (SMALL) {
+                        // the columns of heads 4 to 7 hold the other 16 keys: what they give is not looked at
+                        pb[n][0][key] = transpose8(two);
+                        pb[n][1][key] = transpose8(__shfl_xor_sync(0xffffffffu, two, 2));
+                    } else {
+                        pb[n][key >> 1][key & 1] = transpose8(two);
+                    }
                 }
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                uint32_t w[4];
+                uint32_t w[4], low[4], both[4];
                 ldsm4_trans(w, row_at + 128 * (NC + c));
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
+                for (int half = 0; half < 2; ++half) {
+                    codes(w, half, low, both);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
-                            mma(o[n][c][m], w[2 * t] & 0x000f000fu, w[2 * t] & 0x00f000f0u, w[2 * t + 1] & 0x000f000fu, w[2 * t + 1] & 0x00f000f0u,
-                                pb[n][t][0], pb[n][t][1]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] >>= 8;
+                            mma(o[n][c][half], low[2 * t], both[2 * t], low[2 * t + 1], both[2 * t + 1], pb[n][t][0], pb[n][t][1]);
                 }
             }
             }
@@ -503,11 +525,11 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
+                for (int off = SMALL ? 2 : 4; off < 32; off <<= 1) {
                     l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], off);
                     base_v[n][i] += __shfl_xor_sync(0xffffffffu, base_v[n][i], off);
                 }
-                if (g8 == 0) {
+                if (g8 == 0 && (!SMALL || c4 < 2)) {
                     const int h = warp * Z::HEADS + 8 * n + 2 * c4 + i;
                     sM[h] = ref[n][i];
                     sL[h] = worked ? l[n][i] : 0.f;
@@ -518,7 +540,7 @@ kv4_decode_kernel(const Args a) {
         int* s_stage = s_last + 1;                                                   // [WARPS] the stage a warp's sums lie in, -1: it had no keys
         if (lane == 0) s_stage[warp] = worked ? my_stage : -1;
         for (int n = 0; n < NT; ++n) {
-            if (worked) {
+            if (worked && (!SMALL || c4 < 2)) {
                 // sums of 8 heads over the tile just read (its stage is fetched into only after the next tile's wait)
                 float* dst = reinterpret_cast<float*>(my_ring + my_stage * Z::STAGE);
 #pragma unroll
@@ -533,7 +555,7 @@ kv4_decode_kernel(const Args a) {
                     }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < 8 * 8 * NC; i += THREADS) {
+            for (int i = threadIdx.x; i < MERGED * 8 * NC; i += THREADS) {
                 const int h8 = i / (8 * NC), d = 4 * (i % (8 * NC)), h = 8 * n + h8;
                 float m = -INFINITY;
 #pragma unroll
@@ -554,11 +576,11 @@ kv4_decode_kernel(const Args a) {
                     sum = fmaf(f, sL[w * Z::HEADS + h], sum);
                     mins = fmaf(f, sB[w * Z::HEADS + h], mins);
                 }
-                // codes entered as n 2^-24, those in the high four bits of a byte as 16 n 2^-24
+                // sums of n0 2^-24 and of (n0 + 16 n1) 2^-24
+                acc.y = fmaf(acc.y - acc.x, 1048576.f, mins);
                 acc.x = fmaf(acc.x, 16777216.f, mins);
-                acc.y = fmaf(acc.y, 1048576.f, mins);
+                acc.w = fmaf(acc.w - acc.z, 1048576.f, mins);
                 acc.z = fmaf(acc.z, 16777216.f, mins);
-                acc.w = fmaf(acc.w, 1048576.f, mins);
                 if (whole) {
                     if (h < heads && d < a.hd) {
                         const float inv = 1.f / sum;
@@ -665,26 +687,26 @@ kv4_decode_kernel(const Args a) {
     }
 }
 
-template <int NC, int NT> constexpr size_t smem_bytes() {
-    using Z = Sizes<NC, NT>;
+template <int NC, int NT, bool SMALL> constexpr size_t smem_bytes() {
+    using Z = Sizes<NC, NT, SMALL>;
     return (size_t)WARPS * Z::STAGES * Z::STAGE + WARPS * Z::STAGES * 8 + 3 * WARPS * Z::HEADS * 4 + 4 * (2 + WARPS);
 }
 
-template <int NC, int NT> int launch(const Args& a, long long max_rounds, int sms, long long partial_floats, cudaStream_t stream) {
-    using Z = Sizes<NC, NT>;
+template <int NC, int NT, bool SMALL = false> int launch(const Args& a, long long max_rounds, int sms, long long partial_floats, cudaStream_t stream) {
+    using Z = Sizes<NC, NT, SMALL>;
     if (partial_floats < 2LL * sms * Z::BLOCKS * Z::PARTIAL) return VOB_ERR_BAD_ARG;
     static char done[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(kv4_decode_kernel<NC, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NC, NT>());
+        e = cudaFuncSetAttribute(kv4_decode_kernel<NC, NT, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<NC, NT, SMALL>());
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) done[dev] = 1;
     }
     const long long most = (long long)a.S * a.G * a.head_tiles * max_rounds;
     const int grid = (int)min(most, (long long)sms * Z::BLOCKS);
-    return vob_launch(kv4_decode_kernel<NC, NT>, dim3(max(grid, 1)), dim3(THREADS), smem_bytes<NC, NT>(), stream, a);
+    return vob_launch(kv4_decode_kernel<NC, NT, SMALL>, dim3(max(grid, 1)), dim3(THREADS), smem_bytes<NC, NT, SMALL>(), stream, a);
 }
 
 int heads_per_unit(int group, int hd) { return group > 8 && hd <= 128 ? 16 : 8; }
@@ -710,19 +732,29 @@ VOB_EXPORT int vob_kv4_decode(const void* q, long long q_stride, void* out, long
     const long long rounds = keys / (STEP * WARPS) + 2;                              // of the shortest that a size has
     if ((long long)max_pages * page_size > 0x7ffffff0LL || rounds * S * G * a.head_tiles > 0x7fffffffLL) return VOB_ERR_UNSUPPORTED;
     a.table_keys = max_pages * page_size;
-    switch (chunks(hd) * 2 + (heads == 16)) {
-        case 2: return launch<1, 1>(a, rounds, sms, partial_floats, stream);
-        case 3: return launch<1, 2>(a, rounds, sms, partial_floats, stream);
-        case 4: return launch<2, 1>(a, rounds, sms, partial_floats, stream);
-        case 5: return launch<2, 2>(a, rounds, sms, partial_floats, stream);
-        case 6: return launch<3, 1>(a, rounds, sms, partial_floats, stream);
-        case 7: return launch<3, 2>(a, rounds, sms, partial_floats, stream);
-        case 8: return launch<4, 1>(a, rounds, sms, partial_floats, stream);
-        case 9: return launch<4, 2>(a, rounds, sms, partial_floats, stream);
-        case 10: return launch<5, 1>(a, rounds, sms, partial_floats, stream);
-        case 12: return launch<6, 1>(a, rounds, sms, partial_floats, stream);
-        case 14: return launch<7, 1>(a, rounds, sms, partial_floats, stream);
-        case 16: return launch<8, 1>(a, rounds, sms, partial_floats, stream);
+    const bool small = H / G <= 4;
+#define VOB_DECODE(NC)                                                                                              \
+    case NC:                                                                                                        \
+        return small ? launch<NC, 1, true>(a, rounds, sms, partial_floats, stream) : launch<NC, 1>(a, rounds, sms, partial_floats, stream);
+    if (heads == 16) {
+        switch (chunks(hd)) {
+            case 1: return launch<1, 2>(a, rounds, sms, partial_floats, stream);
+            case 2: return launch<2, 2>(a, rounds, sms, partial_floats, stream);
+            case 3: return launch<3, 2>(a, rounds, sms, partial_floats, stream);
+            case 4: return launch<4, 2>(a, rounds, sms, partial_floats, stream);
+        }
+        return VOB_ERR_UNSUPPORTED;
     }
+    switch (chunks(hd)) {
+        VOB_DECODE(1)
+        VOB_DECODE(2)
+        VOB_DECODE(3)
+        VOB_DECODE(4)
+        VOB_DECODE(5)
+        VOB_DECODE(6)
+        VOB_DECODE(7)
+        VOB_DECODE(8)
+    }
+#undef VOB_DECODE
     return VOB_ERR_UNSUPPORTED;
 }
