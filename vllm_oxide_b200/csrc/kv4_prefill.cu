@@ -1,15 +1,22 @@
 // Attention of portions of prompts over the 4-bit cache (layout: kv4.cuh) on the 5th-generation tensor cores: bfloat16 activations, head sizes
 // up to 128, any window, any page size, up to 128 heads per kv head.
 //
-// Math: s_j = scale q . K_j over the keys a row sees, softmax in float32 with a running maximum, out = sum_j softmax_j V_j, with
-// K_j = m + s n in bfloat16 (a code n in 0 .. 15 is exact in bfloat16, and m + s n is rounded once, 2^-8 of it), P in bfloat16. A row has
-// dozens to thousands of keys that share a tile's conversion, so here the codes become numbers once per tile and not scores once per row.
+// Math: s_j = scale q . K_j over the keys a row sees, softmax in float32, out = sum_j softmax_j V_j. A row has dozens to thousands of keys that share a
+// tile's conversion, so here the codes become numbers m + s n once per tile, and not scores once per row. Operands are float16, which keeps 11 bits of a
+// number (bfloat16's 8 would double the result's error), with exponents of their own, so that the range is bfloat16's:
+//   * every 32 keys have a power of two for K and one for V that bring their largest number to 2^-7 .. 2^-6 (numbers 2^-18 below that are rounded to
+//     multiples of 2^-19 of it); K's goes into the scale of these keys' scores, V's into the exponent of P, P V being what it was;
+//   * q is a bfloat16 and fits, times a power of two per row;
+//   * P = 2^(score - reference + V's exponent) is rounded to 11 bits; its sum, without V's exponent, is float32. (Where all of 32 keys' values
+//     are below 2^-30, they keep steps of 2^-48. A row that sees values above 2^84, 2e25, loses weights of keys whose values are that much smaller.)
+// With the numbers this small a code needs no conversion: four bits alone in the low mantissa of a float16 are n 2^-24, a subnormal, four bits
+// higher 16 n 2^-24, and one FMA with s 2^24 makes m + s n of it, rounded once.
 //
 // One block: two tiles of 128 rows (token, head of the group) of one request and kv head, over tiles of 128 keys that both share:
 //   * four warps each make the numbers of K and of V: a thread takes a key, its codes already in registers (fetched a tile ahead straight from the
-//     pages, 128 contiguous bytes per eight keys), and writes K and V as bfloat16 into the swizzled operand tiles: per 8 codes 3 shifts,
-//     4 and-ors (a code in the low mantissa bits of 128 is 128 + n), 4 subtractions, 4 FMAs and one 16-byte store. The pairs that this gives are numbers
-//     (0,4), (1,5), (2,6), (3,7) of every eight; they stay in that order in the tiles, q is laid out likewise and the sums are put back at the end;
+//     pages, 128 contiguous bytes per eight keys), and writes them as float16 into the swizzled operand tile: per 8 codes a shift, 4 masks, 4 FMAs and one
+//     16-byte store. The pairs that this gives are numbers (0,4), (1,5), (2,6), (3,7) of every eight; they stay in that order in the tiles, q is laid out
+//     likewise and the sums are put back at the end;
 //   * a thread for each row tile issues its S = Q K^T and O += P V in steps of 64 keys (tcgen05.mma; S, P and O in tensor memory: two S of 64 columns per row
 //     tile, P over its S, O0, O1). The scores of step u + 2 are asked for once P V of step u is done, while the rows
 //     work on step u + 1;
@@ -20,6 +27,7 @@
 // Every wait is bounded (sm100.cuh); on expiry the block raises the error flag, frees its tensor memory and returns.
 #include "kv4.cuh"
 VOB_PDL_SWITCH(kv4_prefill)
+#include <cuda_fp16.h>
 #include "sm100.cuh"
 
 namespace {
@@ -74,20 +82,30 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-// Eight codes -> m + s n as bfloat16, in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ uint4 numbers(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 m) {
-    const __nv_bfloat162 off = __floats2bfloat162_rn(128.f, 128.f);
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// Eight codes -> m + s n as float16, in the order 0 4 1 5 2 6 3 7; `s` and `s16` are s 2^24 and s 2^20.
+__device__ __forceinline__ uint4 numbers(uint32_t w, __half2 s, __half2 s16, __half2 m) {
+    const uint32_t h = w >> 8;
+    const uint32_t t[4] = {w & 0x000f000fu, w & 0x00f000f0u, h & 0x000f000fu, h & 0x00f000f0u};
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t t = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;
-        const __nv_bfloat162 x = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), off), s, m);
+        const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&t[i]), i & 1 ? s16 : s, m);
         r[i] = *reinterpret_cast<const uint32_t*>(&x);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
+// kind::f16 with A and B float16, D float32, both K-major or B MN-major (the bfloat16 form's descriptor without its two format bits).
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, bool b_mn_major) {
+    return umma_idesc_bf16(m, n, b_mn_major) & ~((1u << 7) | (1u << 10));
+}
+// 2^e, -126 <= e <= 127
+__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-template <int HD> constexpr size_t smem_bytes() { return 1024 + (size_t)(2 + 2 + 2) * (HD / 64) * SPAN + 256; }
+template <int HD> constexpr size_t smem_bytes() { return 1024 + (size_t)(2 + 2 + 2) * (HD / 64) * SPAN + 512; }
 
 template <int HD>
 __global__ void __launch_bounds__(NTHREADS, 1)
@@ -118,7 +136,11 @@ kv4_prefill_kernel(const Args a) {
     uint64_t* p_ready = bars + 14;           // [2][2] the tile's 128 rows have written P over them
     uint64_t* o_full = bars + 18;            // [2] a row tile's O holds a step
     uint64_t* o_done = bars + 20;            // [2] and all of them (a barrier of its own: who waits for a phase must know that the one before it has passed)
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 22);
+    uint64_t* scales = bars + 22;            // [4] the powers of two of a key tile are there (a ring of four: rows may still read those of the tile
+                                             //     before the one whose numbers overwrite its stage)
+    float* power = reinterpret_cast<float*>(bars + 26);                // [4 tiles][3][4 times 32 keys]: what K's numbers were divided by; log2 of what V's
+                                                                       // were, and one over that
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(power + 48);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,6 +174,8 @@ kv4_prefill_kernel(const Args a) {
             mbar_init(p_ready + 2 + i, 128);
             mbar_init(o_full + i, 1);
             mbar_init(o_done + i, 1);
+            mbar_init(scales + i, 8);
+            mbar_init(scales + 2 + i, 8);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -171,7 +195,7 @@ kv4_prefill_kernel(const Args a) {
         regs_down<REGS_ISSUE>();
         const int t = warp - 16;                                          // a thread issues the products of one row tile
         if (t < 2 && elect_one()) {
-            constexpr uint32_t idesc_qk = umma_idesc_bf16(BM, BS, false), idesc_pv = umma_idesc_bf16(BM, HD, true);
+            constexpr uint32_t idesc_qk = umma_idesc_f16(BM, BS, false), idesc_pv = umma_idesc_f16(BM, HD, true);
             const int t_from = t ? from[1] : from[0], t_to = t ? to[1] : to[0];
             const uint32_t tS = tmem + t * BN, tO = tmem + 2 * BN + t * HD;
             bool ok = true;
@@ -184,6 +208,9 @@ kv4_prefill_kernel(const Args a) {
                 mbar_arrive(k_free + s);
                 mbar_arrive(v_free + s);
             };
+            // Rows read a tile's powers of two behind its scores; here they are waited for before these are asked for. (128 rows waiting for this barrier
+            // as well took 348 us instead of 332 for 2,048 tokens behind 8,192 at 32/8 heads of 128.)
+            auto wait_scales = [&](int m) { ok = ok && mbar_wait(scales + (m & 3), (m >> 2) & 1, abort_flag, a.err, 51); };
             auto issue_qk = [&](int u) {
                 const int m = (u >> 1) - j0, s = m & 1, b = u & 1;
                 if (!b) ok = ok && mbar_wait(k_full + s, (m >> 1) & 1, abort_flag, a.err, 42);
@@ -202,12 +229,16 @@ kv4_prefill_kernel(const Args a) {
             for (int j = j0; j < j_from && ok; ++j) skip(j);
             if (t_from < t_to) {
                 ok = ok && mbar_wait(q_ready + t, 0, abort_flag, a.err, 43);
+                wait_scales(t_from / 2 - j0);
                 issue_qk(t_from);
                 if (t_from + 1 < t_to) issue_qk(t_from + 1);
             }
             for (int u = t_from; u < t_to && ok; ++u) {
                 const int m = (u >> 1) - j0, s = m & 1, b = u & 1, n = u - t_from;
-                if (!b) ok = mbar_wait(v_full + s, (m >> 1) & 1, abort_flag, a.err, 44);
+                if (!b) {
+                    ok = mbar_wait(v_full + s, (m >> 1) & 1, abort_flag, a.err, 44);
+                    if (u + 2 < t_to) wait_scales(m + 1);
+                }
                 ok = ok && mbar_wait(p_ready + 2 * t + b, (n >> 1) & 1, abort_flag, a.err, 45);
                 if (!ok) break;
                 tcgen05_fence_after();
@@ -271,7 +302,18 @@ kv4_prefill_kernel(const Args a) {
             if (page >= 0) attend_scales(par, ks, vs);
             else if (page == -1) ks = make_float2(NAN, NAN);
             const float2 sm = is_v ? vs : ks;
-            const __nv_bfloat162 s2 = __float2bfloat162_rn(sm.x), m2 = __float2bfloat162_rn(sm.y);
+            // the exponent that the warp's 32 keys share: their largest number is below 2^(exponent - 6)
+            const float most = fmaxf(fabsf(sm.y), fabsf(fmaf(15.f, sm.x, sm.y)));
+            const int top = (int)(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u) >> 23) - 127;
+            const int e = min(max(top + 7, is_v ? -24 : -50), 126);
+            const float down = power2(-e);
+            const __half2 m2 = __float2half2_rn(sm.y * down), s2 = __float2half2_rn(sm.x * down * 16777216.f), s16 = __float2half2_rn(sm.x * down * 1048576.f);
+            if ((i & 31) == 0) {
+                float* to = power + ((j - j0) & 3) * 12 + (i >> 5);
+                if (is_v) { to[4] = (float)e; to[8] = down; }
+                else to[0] = power2(e);
+                mbar_arrive(scales + ((j - j0) & 3));
+            }
             // a stage is free once the products of the tile before the last are done
             if (!mbar_wait(free_ + s, (((j - j0) >> 1) & 1) ^ 1, abort_flag, a.err, 46)) break;
             unsigned char* row = tiles + s * TILE + i * 128;
@@ -280,7 +322,7 @@ kv4_prefill_kernel(const Args a) {
                 const uint32_t code[4] = {r[c].x, r[c].y, r[c].z, r[c].w};
 #pragma unroll
                 for (int u = 0; u < 4; ++u)                               // 16 bytes of the row's 128, swizzled by the row
-                    *reinterpret_cast<uint4*>(row + (c >> 1) * SPAN + (((4 * (c & 1) + u) ^ (i & 7)) << 4)) = numbers(code[u], s2, m2);
+                    *reinterpret_cast<uint4*>(row + (c >> 1) * SPAN + (((4 * (c & 1) + u) ^ (i & 7)) << 4)) = numbers(code[u], s2, s16, m2);
             }
             fence_proxy_async_smem();
             mbar_arrive(full + s);
@@ -300,17 +342,34 @@ kv4_prefill_kernel(const Args a) {
         const int last_pos = ctx + (min(total_rows, first_row + (t + 1) * tile_rows) - 1) / group;
         const long long at = (long long)(row0 + rr / group);
         const int head = kvh * group + rr % group;
+        float row_scale = 0.f;                                           // of scores: scale log2 e and what q was divided by
         if (t_to > t_from) {
-            // Q: numbers (0,4), (1,5), (2,6), (3,7) of every eight, as the keys' tiles have them
+            // Q: numbers (0,4), (1,5), (2,6), (3,7) of every eight, as the keys' tiles have them, the row's largest brought to 2^14 .. 2^15
             const uint4* src = reinterpret_cast<const uint4*>(a.q + at * a.q_stride + (size_t)head * a.hd);
             unsigned char* row = sQ + t * TILE + r * 128;
+            uint32_t most = 0;                                           // of two bfloat16 without their signs
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c)
+                if (valid && 8 * c < a.hd) {
+                    const uint4 x = src[c];
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+                }
+            most = max(most & 0xffffu, most >> 16) >> 7;                 // the exponent's bits
+            const int e = most == 255u ? 0 : max((int)most - 127 - 14, -50);    // (not lower: a product of two such scales must not become 0)
+            const float down = power2(-e);
+            row_scale = a.scale_log2 * power2(e);
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (valid && 8 * c < a.hd) x = src[c];
-                const uint4 y = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
-                                           __byte_perm(x.y, x.w, 0x7632));
-                *reinterpret_cast<uint4*>(row + (c >> 3) * SPAN + (((c & 7) ^ (r & 7)) << 4)) = y;
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16) * down; f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * down; }
+                *reinterpret_cast<uint4*>(row + (c >> 3) * SPAN + (((c & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(pack_half(f[0], f[4]), pack_half(f[1], f[5]), pack_half(f[2], f[6]), pack_half(f[3], f[7]));
             }
             fence_proxy_async_smem();
             mbar_arrive(q_ready + t);
@@ -332,6 +391,9 @@ kv4_prefill_kernel(const Args a) {
             uint32_t va[32], vb[32];
             tmem_ld32(tS, va);
             tmem_ld32(tS + 32, vb);
+            const float2* pw = reinterpret_cast<const float2*>(power + (((u >> 1) - j0) & 3) * 12 + 2 * b);       // (the issue of the scores waited for them)
+            const float2 kp = pw[0], ev = pw[2], v_inv = pw[4];
+            const float sc_a = row_scale * kp.x, sc_b = row_scale * kp.y;
             tmem_wait_ld();
             if (masked) {
                 const int see_from = a.window ? pos - a.window + 1 - kbase : -0x7fffffff, see_to = pos - kbase;      // keys of the step that the row sees
@@ -341,43 +403,42 @@ kv4_prefill_kernel(const Args a) {
                     if (i + 32 > see_to || i + 32 < see_from) vb[i] = 0xff800000u;
                 }
             }
-            // P = 2^(score - m_ref) over the scores, and their sum. m_ref is some maximum of earlier steps: as long as no row's sum passes 2^10 it
-            // may stay, since P, the sums and O are floating-point numbers relative to it.
-            const float2 sc2 = make_float2(a.scale_log2, a.scale_log2);
-            float sum;
-            auto weigh = [&]() {
-                const float2 nm2 = make_float2(-m_ref, -m_ref);
-                float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-                auto half = [&](const uint32_t (&v)[32], float2& acc, uint32_t to_column) {
-                    uint32_t pk[16];
+            // P = 2^(score - m_ref + V's exponent) over the scores, and their sums. m_ref is some maximum of earlier steps: as long as no row's sum passes
+            // 2^10 it may stay, since P, the sums and O are floating-point numbers relative to it.
+            float sum_a, sum_b;
+            auto half = [&](const uint32_t (&v)[32], float sc, float shift, uint32_t to_column) {
+                const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(shift - m_ref, shift - m_ref);
+                float2 acc = make_float2(0.f, 0.f);
+                uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
-                        const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                        acc = __fadd2_rn(acc, p);
-                        pk[i >> 1] = pack_bf16(p.x, p.y);
-                    }
-                    tmem_st16(tS + to_column, pk);                        // over scores that are in registers
-                };
-                half(va, acc0, 0);
-                half(vb, acc1, 16);
-                sum = (acc0.x + acc0.y) + (acc1.x + acc1.y);
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
+                    const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                    acc = __fadd2_rn(acc, p);
+                    pk[i >> 1] = pack_half(p.x, p.y);
+                }
+                tmem_st16(tS + to_column, pk);                            // over scores that are in registers
+                return acc.x + acc.y;
+            };
+            auto weigh = [&]() {
+                sum_a = half(va, sc_a, ev.x, 0);
+                sum_b = half(vb, sc_b, ev.y, 16);
             };
             bool move = n == 0;
             if (!move) {
                 weigh();
-                move = __any_sync(0xffffffffu, !(sum <= 1024.f));
+                move = __any_sync(0xffffffffu, !(sum_a + sum_b <= 1024.f));
             }
             if (move) {
                 float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    mx0 = max3(mx0, __uint_as_float(va[i]), __uint_as_float(vb[i]));
-                    mx1 = max3(mx1, __uint_as_float(va[i + 1]), __uint_as_float(vb[i + 1]));
+                    mx0 = max3(mx0, __uint_as_float(va[i]), __uint_as_float(va[i + 1]));
+                    mx1 = max3(mx1, __uint_as_float(vb[i]), __uint_as_float(vb[i + 1]));
                 }
-                mx0 = max3(mx0, mx1, mx1);
-                nan_row = nan_row || mx0 != mx0;
-                const float m_new = fmaxf(m_ref, mx0 * a.scale_log2);    // scale > 0: the maximum commutes. NaN: m_ref stays
+                nan_row = nan_row || mx0 != mx0 || mx1 != mx1;
+                // the scales are positive: the maximum commutes. NaN: m_ref stays
+                const float m_new = fmaxf(m_ref, fmaxf(fmaf(mx0, sc_a, ev.x), fmaf(mx1, sc_b, ev.y)));
                 const float alpha = m_ref < m_new ? exp2_fast(m_ref - m_new) : 1.f;       // m_ref = -inf: 0
                 m_ref = m_new == -INFINITY ? FLT_LOWEST : m_new;         // a row that has seen nothing: 2^(-inf + that) = 0
                 l *= alpha;
@@ -400,7 +461,7 @@ kv4_prefill_kernel(const Args a) {
             tmem_wait_st();
             tcgen05_fence_before();
             mbar_arrive(p_ready + 2 * t + b);
-            l += sum;
+            l = fmaf(sum_a, v_inv.x, fmaf(sum_b, v_inv.y, l));
         }
         if (ok && t_to > t_from && wait_all(o_done + t, 0, 50)) {
             tcgen05_fence_after();
