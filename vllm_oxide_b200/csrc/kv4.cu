@@ -326,11 +326,14 @@ struct Batch {
     float scale;
 };
 
-// Eight codes as numbers: a code in the low bits of 2^23 is 2^23 + n.
-__device__ __forceinline__ float code_number(uint32_t w, int i) { return __uint_as_float((w >> (4 * i) & 15u) | 0x4b000000u) - 8388608.f; }
+// Eight codes as numbers n - 8: a code in the low bits of 2^23 is 2^23 + n. Sums over codes about 0 are as small as what they stand for, those over 0 to
+// 15 are not, and their rounding shows where the minimum's share is taken off again (1.1e-6 of the result instead of what is given at the kernel).
+template <int ZERO = 8> __device__ __forceinline__ float code_number(uint32_t w, int i) {
+    return __uint_as_float((w >> (4 * i) & 15u) | 0x4b000000u) - (8388608.f + ZERO);
+}
 
 // Single tokens. A block has 4 heads of one request and kv head, and `splits` blocks share the request's keys; each of its warps takes 32 keys at a time, by
-// itself: a lane a key for the scores, sum(q n) s + m sum(q) on the codes as they come from the cache, then two numbers a lane (NB times 64 numbers) for the
+// itself: a lane a key for the scores, sum(q (n - 8)) s + (m + 8 s) sum(q) on the codes as they come from the cache, then two numbers a lane (NB times 64 numbers) for the
 // sums, the codes of the values going through shared memory. The warps' results meet at the end, the blocks' in the block that arrives last, in the
 // order of the keys. Bound: instructions (some 16 per key and 32 lanes for the scores, as many for the sums, at 4 heads of 64).
 constexpr int SINGLE_ROWS = 4, SINGLE_WARPS = 4;
@@ -395,6 +398,8 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
             if (page >= 0 && page < b.num_pages) {
                 grp = cache + group_at(page, g, off, b.G, b.page_size, width) + (off & 7) * 16;
                 attend_scales(*reinterpret_cast<const uint2*>(grp + 256 * C - (off & 7) * 8), ks, vs);
+                ks.y = fmaf(8.f, ks.x, ks.y);               // what code 8 stands for
+                vs.y = fmaf(8.f, vs.x, vs.y);
             } else {
                 ks = make_float2(NAN, NAN);                 // a page outside the pool: the rows that see it become NaN
             }
@@ -513,157 +518,238 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
     }
 }
 
-// Portions. One block: ROWS rows (token, head of the group) of one request and kv head, over KEYS keys at a time: codes become numbers in
-// shared memory once per tile, each of 256 threads takes 4 rows x 1 key of the scores and 4 rows x DP / 64 numbers of the sums, the maximum
-// and the sum of a row run along in shared memory.
-// Bound: the FMA pipe's operands in shared memory.
-constexpr int ROWS = 16, KEYS = 64, FLEX_THREADS = 256;
+// Portions. One block: 16 R rows (token, head of the group) of one request and kv head, over KEYS keys at a time. Codes become numbers in shared memory once
+// per tile (fetched a tile ahead). A thread has R rows x 4 keys of the scores (16 threads share a row), the rows' maxima and sums and R rows x DP / 16
+// numbers of the sums in registers; the probabilities cross over within its warp. Where there are few rows a cluster of blocks shares their keys.
+// Bound: the FMA pipe at R = 4 (a tile's 64 keys x 4 rows take 2 x 4 x 64 FMAs a thread and 64 numbers, and 3/4 of the shared memory's
+// time), shared memory at R = 1, which is for requests of few rows.
+constexpr int KEYS = 64, FLEX_THREADS = 256, MIN_TILES = 2;            // tiles of keys that a block of a cluster has at least
 
-template <int DP> constexpr size_t flex_smem() {
-    return sizeof(float) * ((size_t)KEYS * (DP + 4) + (size_t)KEYS * DP + ROWS * DP + KEYS * ROWS + 3 * ROWS);
+template <int DP, int R> constexpr size_t flex_smem() {
+    return sizeof(float) * ((size_t)(2 * KEYS + 16 * R) * (DP + 4) + (size_t)KEYS * (16 * R + 4));
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(FLEX_THREADS)
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(FLEX_THREADS, DP == 64 ? (R == 1 ? 4 : 2) : DP == 128 && R == 1 ? 2 : 1)
 kv4_attend_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const unsigned char* __restrict__ cache,
                   Batch b) {
+    constexpr int ROWS = 16 * R, LD = DP + 4, LP = ROWS + 4, ND = DP / 64, CM = DP / 32;
     extern __shared__ float4 smem4[];
-    float* sK = reinterpret_cast<float*>(smem4);           // [KEYS][DP + 4]
-    float* sV = sK + KEYS * (DP + 4);                      // [KEYS][DP]
-    float* sQ = sV + KEYS * DP;                            // [ROWS][DP]
-    float* sP = sQ + ROWS * DP;                            // [KEYS][ROWS]
-    float* sM = sP + KEYS * ROWS;                          // [ROWS] running maximum
-    float* sL = sM + ROWS;                                 // [ROWS] running sum
-    float* sA = sL + ROWS;                                 // [ROWS] factor of this tile for what came before
+    float* sK = reinterpret_cast<float*>(smem4);           // [KEYS][LD]
+    float* sV = sK + KEYS * LD;                            // [KEYS][LD]
+    float* sQ = sV + KEYS * LD;                            // [ROWS][LD]
+    float* sP = sQ + ROWS * LD;                            // [KEYS][LP]
     pdl_launch_dependents();
     pdl_wait(32);
+    const int parts = (int)cluster_blocks(), rank = (int)cluster_rank();
     const int seq = blockIdx.z, g = blockIdx.y;
     const int group = b.H / b.G, hd = b.hd, tid = threadIdx.x;
     const int row0 = b.seq_starts[seq], tokens = b.seq_starts[seq + 1] - row0, ctx = b.context_lens[seq];
-    const int total = tokens * group, tile0 = blockIdx.x * ROWS;
+    const int total = tokens * group, tile0 = (gridDim.x / parts - 1 - blockIdx.x / parts) * ROWS;       // later rows, which see more keys, start first
     if (tile0 >= total) return;
     const int nrows = min(ROWS, total - tile0);
     const int last_tok = (tile0 + nrows - 1) / group, first_tok = tile0 / group;
     const int hi = ctx + last_tok + 1;                                                    // keys any row sees: [lo, hi)
     const int lo = b.window ? max(0, ctx + first_tok - b.window + 1) : 0;
-    const int t0 = lo / KEYS, t1 = (hi + KEYS - 1) / KEYS;                               // tiles of keys
+    const int t_lo = lo / KEYS, t_hi = (hi + KEYS - 1) / KEYS, share = max(MIN_TILES, (t_hi - t_lo + parts - 1) / parts);
+    const int used = (t_hi - t_lo + share - 1) / share;                                  // blocks of the cluster that have keys
+    const int t0 = t_lo + rank * share, t1 = min(t_hi, t0 + share);
+    if (used == 1 && rank) return;
+    const int rg = (tid >> 4) * R, kl = tid & 15;
+    const float scale = b.scale * 1.4426950408889634f;                                    // probabilities are powers of two
     for (int i = tid; i < ROWS * DP; i += FLEX_THREADS) {
         const int r = i / DP, d = i % DP, rr = tile0 + r;
-        sQ[i] = (r < nrows && d < hd) ? ld_f(q + (size_t)(row0 + rr / group) * q_stride + (size_t)(g * group + rr % group) * hd + d) * b.scale : 0.f;
+        sQ[r * LD + d] = (r < nrows && d < hd) ? ld_f(q + (size_t)(row0 + rr / group) * q_stride + (size_t)(g * group + rr % group) * hd + d) * scale : 0.f;
     }
-    if (tid < ROWS) { sM[tid] = -INFINITY; sL[tid] = 0.f; }
-    constexpr int ND = DP / 64;                            // numbers of the sums per thread and row
-    float acc[4][ND];
+    float acc[R][4 * ND], m[R], l[R];
+    int pos[R];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        pos[r] = rg + r < nrows ? ctx + (tile0 + rg + r) / group : -1;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[r][d] = 0.f;
-    const int key = tid & 63, rg = (tid >> 6) * 4;
+        for (int d = 0; d < 4 * ND; ++d) acc[r][d] = 0.f;
+    }
     const int C = chunks(hd), width = token_bytes(hd);
     const int* bt = b.block_tables + (size_t)seq * b.max_pages;
-
+    // four threads a key, each four bytes (8 codes) of every chunk
+    const int kk = tid >> 2, part = tid & 3;
+    uint32_t kn[CM], vn[CM];
+    float2 ks, vs;
+    auto fetch = [&](int tile) {
+        const int j = tile * KEYS + kk;
+        ks = vs = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < CM; ++c) kn[c] = vn[c] = 0u;
+        if (tile >= t1 || j >= hi || j < lo) return;
+        const int pi = j / b.page_size, off = j - pi * b.page_size;
+        const int page = pi < b.max_pages ? bt[pi] : -1;
+        if (page < 0 || page >= b.num_pages) {
+            ks = make_float2(NAN, NAN);                     // a page outside the pool: the rows that see it become NaN
+            return;
+        }
+        const unsigned char* grp = cache + group_at(page, g, off, b.G, b.page_size, width) + (off & 7) * 16;
+#pragma unroll
+        for (int c = 0; c < CM; ++c)
+            if (c < C) {
+                kn[c] = *reinterpret_cast<const uint32_t*>(grp + c * 128 + part * 4);
+                vn[c] = *reinterpret_cast<const uint32_t*>(grp + (C + c) * 128 + part * 4);
+            }
+        attend_scales(*reinterpret_cast<const uint2*>(grp + 256 * C - (off & 7) * 8), ks, vs);
+    };
+    fetch(t0);
     for (int tile = t0; tile < t1; ++tile) {
         __syncthreads();
-        // a warp fetches 8 keys in turn: 4 lanes per key, each C bytes-of-four at a time
-        for (int kk = tid >> 2; kk < KEYS; kk += FLEX_THREADS / 4) {
-            const int j = tile * KEYS + kk, part = tid & 3;
-            float2 ks = make_float2(0.f, 0.f), vs = ks;
-            const unsigned char* grp = nullptr;
-            if (j < hi && j >= lo) {
-                const int pi = j / b.page_size, off = j - pi * b.page_size;
-                const int page = pi < b.max_pages ? bt[pi] : -1;
-                if (page >= 0 && page < b.num_pages) {
-                    grp = cache + group_at(page, g, off, b.G, b.page_size, width) + (off & 7) * 16;
-                    attend_scales(*reinterpret_cast<const uint2*>(grp + 256 * C - (off & 7) * 8), ks, vs);
-                } else {
-                    ks = make_float2(NAN, NAN);             // a page outside the pool: the rows that see it become NaN
-                }
-            }
-            for (int c = 0; c < C; ++c) {
-                const uint32_t kn = grp ? *reinterpret_cast<const uint32_t*>(grp + c * 128 + part * 4) : 0u;
-                const uint32_t vn = grp ? *reinterpret_cast<const uint32_t*>(grp + (C + c) * 128 + part * 4) : 0u;
-                const int d = c * 32 + part * 8;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sK[kk * (DP + 4) + d + i] = fmaf((float)(kn >> (4 * i) & 15), ks.x, ks.y);
-                    sV[kk * DP + d + i] = fmaf((float)(vn >> (4 * i) & 15), vs.x, vs.y);
+        for (int c = 0; c < CM; ++c)
+            if (c < C) {
+                float* to[2] = {sK + kk * LD + c * 32 + part * 8, sV + kk * LD + c * 32 + part * 8};
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t n = w ? vn[c] : kn[c];
+                    const float s = w ? vs.x : ks.x, o = w ? vs.y : ks.y;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        float4 x;
+                        x.x = fmaf(code_number<0>(n, i), s, o);
+                        x.y = fmaf(code_number<0>(n, i + 1), s, o);
+                        x.z = fmaf(code_number<0>(n, i + 2), s, o);
+                        x.w = fmaf(code_number<0>(n, i + 3), s, o);
+                        *reinterpret_cast<float4*>(to[w] + i) = x;
+                    }
                 }
             }
-        }
         __syncthreads();
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        fetch(tile + 1);
+        float s[R][4];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[r][c] = 0.f;
+#pragma unroll 2
         for (int d = 0; d < hd; d += 4) {
-            const float4 kx = *reinterpret_cast<const float4*>(sK + key * (DP + 4) + d);
+            float4 kx[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 qx = *reinterpret_cast<const float4*>(sQ + (rg + r) * DP + d);
-                s[r] = fmaf(kx.w, qx.w, fmaf(kx.z, qx.z, fmaf(kx.y, qx.y, fmaf(kx.x, qx.x, s[r]))));
+            for (int c = 0; c < 4; ++c) kx[c] = *reinterpret_cast<const float4*>(sK + (kl + 16 * c) * LD + d);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float4 qx = *reinterpret_cast<const float4*>(sQ + (rg + r) * LD + d);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[r][c] = fmaf(kx[c].w, qx.w, fmaf(kx[c].z, qx.z, fmaf(kx[c].y, qx.y, fmaf(kx[c].x, qx.x, s[r][c]))));
             }
         }
-        const int j = tile * KEYS + key;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = ctx + (tile0 + rg + r) / group;
-            const bool seen = rg + r < nrows && j <= p && (!b.window || j > p - b.window);
-            sP[key * ROWS + rg + r] = seen ? s[r] : -INFINITY;
-        }
-        __syncthreads();
-        // 16 threads per row: the tile's maximum, the probabilities, their sum
-        {
-            const int r = tid >> 4, i = tid & 15;
-            float x[KEYS / 16], mx = -INFINITY;
+        for (int r = 0; r < R; ++r) {
+            float mx = m[r];
 #pragma unroll
-            for (int n = 0; n < KEYS / 16; ++n) {
-                x[n] = sP[(i + 16 * n) * ROWS + r];
-                mx = fmaxf(mx, x[n]);
+            for (int c = 0; c < 4; ++c) {
+                const int j = tile * KEYS + kl + 16 * c;
+                if (j > pos[r] || (b.window && j <= pos[r] - b.window)) s[r][c] = -INFINITY;
+                mx = fmaxf(mx, s[r][c]);
             }
+#pragma unroll
             for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float m0 = sM[r], m1 = fmaxf(m0, mx), use = m1 == -INFINITY ? 0.f : m1;
-            float sum = 0.f;
+            const float use = mx == -INFINITY ? 0.f : mx, a = m[r] == -INFINITY ? 0.f : exp2f(m[r] - use);
+            m[r] = mx;
+            l[r] *= a;
 #pragma unroll
-            for (int n = 0; n < KEYS / 16; ++n) {
-                const float p = expf(x[n] - use);
-                sP[(i + 16 * n) * ROWS + r] = p;
-                sum += p;
+            for (int c = 0; c < 4; ++c) {
+                s[r][c] = exp2f(s[r][c] - use);
+                l[r] += s[r][c];
             }
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (i == 0) {
-                const float a = m0 == -INFINITY ? 0.f : expf(m0 - use);
-                sA[r] = a;
-                sL[r] = sL[r] * a + sum;
-                sM[r] = m1;
-            }
+#pragma unroll
+            for (int d = 0; d < 4 * ND; ++d) acc[r][d] *= a;
         }
-        __syncthreads();
+        // the rows of a thread are those of its half of the warp: only that crosses over
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float a = sA[rg + r];
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) acc[r][d] *= a;
-        }
-        for (int kk = 0; kk < KEYS; ++kk) {
-            const float4 p = *reinterpret_cast<const float4*>(sP + kk * ROWS + rg);
+            for (int r = 0; r < R; ++r) sP[(kl + 16 * c) * LP + rg + r] = s[r][c];
+        __syncwarp();
+#pragma unroll 4
+        for (int k = 0; k < KEYS; ++k) {
+            float p[R];
+            if constexpr (R == 4) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(sP + k * LP + rg);
+            else p[0] = sP[k * LP + rg];
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const float x = sV[kk * DP + key + 64 * d];
-                acc[0][d] = fmaf(p.x, x, acc[0][d]);
-                acc[1][d] = fmaf(p.y, x, acc[1][d]);
-                acc[2][d] = fmaf(p.z, x, acc[2][d]);
-                acc[3][d] = fmaf(p.w, x, acc[3][d]);
+            for (int i = 0; i < ND; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(sV + k * LD + 4 * kl + 64 * i);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    acc[r][4 * i] = fmaf(p[r], x.x, acc[r][4 * i]);
+                    acc[r][4 * i + 1] = fmaf(p[r], x.y, acc[r][4 * i + 1]);
+                    acc[r][4 * i + 2] = fmaf(p[r], x.z, acc[r][4 * i + 2]);
+                    acc[r][4 * i + 3] = fmaf(p[r], x.w, acc[r][4 * i + 3]);
+                }
             }
         }
     }
-    __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (rg + r < nrows) {
-            const int rr = tile0 + rg + r;
-            const float l = sL[rg + r], inv = l == 0.f ? 0.f : 1.f / l;
-            T* dst = out + (size_t)(row0 + rr / group) * out_stride + (size_t)(g * group + rr % group) * hd;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-                if (key + 64 * d < hd) st_f(dst + key + 64 * d, acc[r][d] * inv);
+        for (int o = 8; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+    auto row = [&](int r) {
+        const int rr = tile0 + r;
+        return out + (size_t)(row0 + rr / group) * out_stride + (size_t)(g * group + rr % group) * hd;
+    };
+    if (used == 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (rg + r < nrows) {
+                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+                T* dst = row(rg + r);
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        if (4 * kl + 64 * i < hd) st_f(dst + 4 * kl + 64 * i + d, acc[r][4 * i + d] * inv);
+            }
+        return;
+    }
+    __syncthreads();                                       // K gives way to the sums, P to the maxima and the weights' sums
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            *reinterpret_cast<float4*>(sK + (rg + r) * LD + 4 * kl + 64 * i) = make_float4(acc[r][4 * i], acc[r][4 * i + 1], acc[r][4 * i + 2], acc[r][4 * i + 3]);
+        if (kl == 0) { sP[rg + r] = m[r]; sP[ROWS + rg + r] = l[r]; }
+    }
+    cluster_sync();
+    const int each = (nrows + parts - 1) / parts, r_end = min(nrows, (rank + 1) * each);
+    for (int i = rank * each * hd + tid; i < r_end * hd; i += FLEX_THREADS) {
+        const int r = i / hd, d = i - r * hd;
+        float all = -INFINITY, sum = 0.f, o = 0.f;
+        for (int c = 0; c < used; ++c) all = fmaxf(all, ld_cluster(sP + r, c));
+        for (int c = 0; c < used; ++c) {
+            const float f = part_weight(ld_cluster(sP + r, c), all);
+            sum = fmaf(f, ld_cluster(sP + ROWS + r, c), sum);
+            o = fmaf(f, ld_cluster(sK + r * LD + d, c), o);
         }
+        st_f(row(r) + d, sum == 0.f ? 0.f : o / sum);
+    }
+    cluster_sync();                                        // no block leaves while others read from it
+}
+
+template <typename T, int DP, int R>
+int launch_portions(const void* q, long long q_stride, void* out, long long out_stride, const unsigned char* cache, const Batch& b, int S, long long tiles,
+                    cudaStream_t stream) {
+    // once per device that the process uses: the attribute belongs to the current one
+    static char done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(kv4_attend_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)flex_smem<DP, R>());
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) done[dev] = 1;
+    }
+    // two blocks an SM or more: fewer leave SMs idle behind the longest (2 requests of up to 700 tokens behind up to 2,000, 8/2 heads of 256: 554 us with one
+    // an SM, 324 with two), more split what two already keep busy (600 tokens, a window of 100: 77 us unsplit, 162 split)
+    const long long sees = min((long long)b.max_pages * b.page_size, b.window ? (long long)b.window + 16 * R : 0x7fffffffLL);
+    const int parts = key_parts(tiles * b.G * S, 296, sees / (MIN_TILES * KEYS));
+    return launch_clusters(kv4_attend_kernel<T, DP, R>, dim3((unsigned)(tiles * parts), b.G, S), parts, dim3(FLEX_THREADS), flex_smem<DP, R>(), stream,
+                           (const T*)q, q_stride, (T*)out, out_stride, cache, b);
 }
 
 template <typename T, int DP>
@@ -675,20 +761,11 @@ int launch_attend(const void* q, long long q_stride, void* out, long long out_st
         return vob_launch(kv4_single_kernel<T, DP / 64>, dim3(splits, (unsigned)units, S), dim3(32 * SINGLE_WARPS), 0, stream, (const T*)q, q_stride,
                           (T*)out, out_stride, cache, b, splits, partials, arrived);
     }
-    // once per device that the process uses: the attribute belongs to the current one
-    static size_t done[64] = {};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(kv4_attend_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)flex_smem<DP>());
-        if (e != cudaSuccess) return (int)e;
-        if (dev < 64) done[dev] = 1;
-    }
-    const long long tiles = ((long long)max_new * (b.H / b.G) + ROWS - 1) / ROWS;
-    if (tiles > 0x7fffffffLL || b.G > 65535 || S > 65535) return VOB_ERR_UNSUPPORTED;
-    return vob_launch(kv4_attend_kernel<T, DP>, dim3((unsigned)tiles, b.G, S), dim3(FLEX_THREADS), flex_smem<DP>(), stream,
-                      (const T*)q, q_stride, (T*)out, out_stride, cache, b);
+    const long long rows = (long long)max_new * (b.H / b.G), tiles = (rows + 15) / 16;
+    if (tiles > 0x0fffffffLL || b.G > 65535 || S > 65535) return VOB_ERR_UNSUPPORTED;
+    // one row a thread where a request's rows would leave half of the threads' four idle, or four would leave SMs without a block
+    if (rows <= 32 || (rows + 63) / 64 * b.G * S * 8 < 148) return launch_portions<T, DP, 1>(q, q_stride, out, out_stride, cache, b, S, tiles, stream);
+    return launch_portions<T, DP, 4>(q, q_stride, out, out_stride, cache, b, S, (rows + 63) / 64, stream);
 }
 
 bool sizes_ok(int H, int G, int hd, int page_size) {

@@ -44,4 +44,51 @@ __device__ __forceinline__ void attend_scales(uint2 p, float2& key, float2& val)
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Blocks that share the keys of a row form a cluster, each with its part of the sums in its own shared memory; at the end every block joins
+// a share of the rows, reading the others'.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_blocks() { uint32_t n; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t n; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n)); return n; }
+// All threads of all its blocks; what they wrote before is seen behind it. No wait here depends on anything but the blocks' own bounded loops.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float of block `rank`'s shared memory, where this block has `p`.
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+    uint32_t at;
+    float x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+    return x;
+}
+// The weight of a part of a row's keys whose maximum (base 2) is `mine`: a part without keys has nothing to weigh (its sums are 0); one whose keys all
+// gave NaN has no maximum either, and stays NaN.
+__device__ __forceinline__ float part_weight(float mine, float all) { return mine == -INFINITY ? 1.f : exp2f(mine - all); }
+
+// Blocks that share a row's keys, up to the 8 of a portable cluster and to `most`, so that there are `wanted` in all.
+static inline int key_parts(long long blocks, long long wanted, long long most) {
+    int n = 1;
+    while (n < 8 && blocks * n < wanted && 2 * n <= most) n *= 2;
+    return n;
+}
+template <typename... P, typename... A>
+static inline int launch_clusters(void (*kernel)(P...), dim3 grid, int parts, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_vob_pdl ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e != cudaSuccess ? (int)e : vob_launch_status();
+}
+
 }  // namespace vob_kv4
