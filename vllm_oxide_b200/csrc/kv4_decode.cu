@@ -28,6 +28,7 @@
 #include "kv4.cuh"
 VOB_PDL_SWITCH(kv4_decode)
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "sm100.cuh"
 
 namespace {
@@ -46,8 +47,8 @@ template <int NC, int NT, bool SMALL> struct Sizes {
     static constexpr int TILE = NC <= 2 ? 64 : 32;                // keys of a stage of a warp's ring: one or two steps
     static constexpr int ROUND = TILE * WARPS;                    // keys that a block takes at a time
     static constexpr int STAGE = SUB * (TILE / GROUP);
-    static constexpr int BLOCKS = NC > 4 || NC * NT > 4 ? 2 : NC * NT == 4 ? 3 : 4 - (NT - 1);
-    static constexpr int STAGES = NC > 4 || NC <= 2 ? 3 : NT == 2 ? 5 : NC == 4 ? 4 : 3;
+    static constexpr int BLOCKS = NC > 4 || NC * NT > 4 ? 2 : NC * NT == 4 || (NC * NT == 3 && !SMALL) ? 3 : 4 - (NT - 1);
+    static constexpr int STAGES = NC > 4 || NC <= 2 ? 3 : NT == 2 ? 5 : NC == 4 || !SMALL ? 4 : 3;
     static constexpr int HEADS = 8 * NT;
     static constexpr int OSTRIDE = 32 * NC + 8;                   // a head's sums in a stage, padded: 8 heads fill it exactly
     static constexpr int PARTIAL = HEADS * (32 * NC + 2);         // floats of a partial result
@@ -69,6 +70,12 @@ struct Args {
     float scale_log2;
 };
 
+// The smaller, NaN if one of them is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -428,12 +435,15 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < KEYS; ++i) vt[i] = fmaxf(vs[i].x, 9.094947e-13f);
             float p[NT][KEYS][2], most = 0.f;                                           // the largest p_j times scale
-            auto weigh = [&](int n) {
+            // `moved`: behind a move a score is rounded before the reference is taken off it, as the reference was, so that the largest keeps its weight however
+            // large scores are; and a product is held to 2^8 (they are 2^4 at most but for the reference's rounding).
+            float lg[KEYS];                                                             // log2 of the value's scale, behind a move
+            auto weigh = [&](auto moved, int n) {
                 float e[KEYS][2];
 #pragma unroll
                 for (int key = 0; key < KEYS; ++key)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) e[key][h] = fmaf(ks[key].y, qs[n][h], -ref[n][h]);
+                    for (int h = 0; h < 2; ++h) e[key][h] = decltype(moved)::value ? ks[key].y * qs[n][h] : fmaf(ks[key].y, qs[n][h], -ref[n][h]);
                 if (edge) {
 #pragma unroll
                     for (int key = 0; key < KEYS; ++key)
@@ -442,15 +452,18 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
                 for (int key = 0; key < KEYS; ++key) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) p[n][key][h] = exp2_fast(fmaf(z[n][key][h], ks[key].x, e[key][h]));
+                    for (int h = 0; h < 2; ++h) {
+                        float x = fmaf(z[n][key][h], ks[key].x, e[key][h]);
+                        if constexpr (decltype(moved)::value) x = min_nan(x - ref[n][h], 4.f - lg[key]);
+                        p[n][key][h] = exp2_fast(x);
+                    }
                     most = fmaxf(most, fmaxf(p[n][key][0], p[n][key][1]) * vt[key]); // (NaN is left out: it stays in p)
                 }
             };
 #pragma unroll
-            for (int n = 0; n < NT; ++n) weigh(n);
+            for (int n = 0; n < NT; ++n) weigh(std::false_type(), n);
             if (__any_sync(0xffffffffu, most > P_LIMIT)) {
                 // a new reference: the largest score + log2 of its value's scale
-                float lg[KEYS];
 #pragma unroll
                 for (int i = 0; i < KEYS; ++i) lg[i] = log2f(vt[i]) - P_TOP;
 #pragma unroll
@@ -477,7 +490,7 @@ kv4_decode_kernel(const Args a) {
 #pragma unroll
                             for (int m = 0; m < 2; ++m) { o[n][c][m][i] *= f; o[n][c][m][2 + i] *= f; }
                     }
-                    weigh(n);
+                    weigh(std::true_type(), n);
                 }
             }
             uint32_t pb[NT][2][2];                                                   // P^T as the B operand
