@@ -325,3 +325,96 @@ def test_a_page_outside_the_pool_makes_its_rows_nan(page_no, dtype):
     kernels.attn_prefill_kv4(q, out, cache, tables[1:2].contiguous(), torch.tensor([0, n], dtype=torch.int32, device=DEV),
                              torch.zeros(1, dtype=torch.int32, device=DEV), 1, n, H, G, hd, hd ** -0.5)
     assert not out[:80].isnan().any() and out[80:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("reqs,H,G,hd,page,window", [
+    # few rows behind long contexts: blocks share the keys, two, four or eight of them, some with none or with one of the two row tiles only
+    ([(5000, 3)], 8, 2, 64, 16, 0), ([(2100, 1)], 4, 4, 128, 16, 0), ([(3000, 90)], 24, 8, 128, 16, 0), ([(2500, 300)], 8, 2, 128, 16, 0),
+    ([(4096, 16), (3, 2)], 8, 2, 64, 16, 0), ([(0, 7), (6000, 9), (70, 0), (1025, 5)], 6, 2, 128, 8, 0), ([(5000, 200)], 8, 1, 64, 16, 1500),
+    ([(2000, 128)], 2, 2, 64, 24, 600), ([(1100, 260)], 4, 4, 128, 16, 700), ([(3000, 40)], 4, 2, 256, 16, 0), ([(1024, 64)], 20, 1, 80, 16, 0)])
+def test_few_rows_behind_long_contexts(reqs, H, G, hd, page, window, dtype):
+    test_portions(reqs, H, G, hd, page, window, dtype)
+
+
+@pytest.mark.parametrize("at", [0, 700, 2047, 4000, 4095])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_nan_token_in_one_blocks_share_of_the_keys(at, dtype):
+    from vllm_oxide_b200 import kernels
+    H, G, hd, page, L, n = 8, 4, 64, 16, 4096, 6
+    g = gen(4)
+    k, v = torch.randn(L, G, hd, generator=g), torch.randn(L, G, hd, generator=g)
+    v[at, 2, 5] = -math.inf                                  # kv head 2: heads 4 and 5
+    cache, kk, vv = plain.pack(k, v, page)
+    tables = torch.arange(L // page, dtype=torch.int32, device=DEV).view(1, -1)
+    q = torch.randn(n, H * hd, generator=g).to(dtype)
+    out = torch.empty(n, H * hd, dtype=dtype, device=DEV)
+    kernels.attn_prefill_kv4(q.to(DEV), out, cache.to(DEV), tables, torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                             torch.tensor([L - n], dtype=torch.int32, device=DEV), 1, n, H, G, hd, hd ** -0.5)
+    got = out.cpu().double().view(n, H, hd)
+    sees = torch.arange(L - n, L) >= at
+    assert got[sees][:, 4:6].isnan().all() and not got[~sees].isnan().any()
+    rest = torch.tensor([0, 1, 2, 3, 6, 7])
+    ref, size, mag = plain.attend(q.view(n, H, hd), kk, vv.nan_to_num(), torch.arange(L - n, L), hd ** -0.5)
+    assert ((got - ref).abs() <= tolerance(ref, size, mag, None, dtype))[:, rest].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd,n", [(64, 200), (128, 300), (96, 20)])
+def test_ranges_far_apart(hd, n, dtype):
+    """Runs of 32 keys whose sizes differ by powers of two up to 2^50, zeros among them, queries of all sizes."""
+    from vllm_oxide_b200 import kernels
+    H, G, page, L = 4, 2, 32, 960
+    g = gen(hd + n)
+    k, v, q = torch.randn(L, G, hd, generator=g), torch.randn(L, G, hd, generator=g), torch.randn(n, H, hd, generator=g)
+    runs = torch.arange(L) // 32
+    # keys small where queries are large, so that scores stay in the range where a softmax has more than one key
+    q[::3] *= 2.0 ** 30
+    q[1::3] *= 2.0 ** -30
+    q[5::7] = 0
+    k *= (2.0 ** torch.randint(-34, 1, (30,), generator=g).float())[runs, None, None]
+    k[::3] *= 2.0 ** -30
+    v *= (2.0 ** torch.randint(-25, 26, (30,), generator=g).float())[runs, None, None]
+    k[64:128], v[96:160], v[8] = 0, 0, 0
+    k, v = (x.to(BF16).float() for x in (k, v))
+    cache, kk, vv = plain.pack(k, v, page)
+    tables = torch.arange(L // page, dtype=torch.int32, device=DEV).view(1, -1)
+    q = q.reshape(n, H * hd).to(dtype)
+    out = torch.empty(n, H * hd, dtype=dtype, device=DEV)
+    kernels.attn_prefill_kv4(q.to(DEV), out, cache.to(DEV), tables, torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                             torch.tensor([L - n], dtype=torch.int32, device=DEV), 1, n, H, G, hd, hd ** -0.5)
+    ref, size, mag = plain.attend(q.view(n, H, hd), kk, vv, torch.arange(L - n, L), hd ** -0.5)
+    # With scores off by e at most, a weight is by a factor of exp(2 e) at most, and what a row gives by (exp(2 e) - 1) mag; e is 2^-8 of the scores' terms
+    # (32 bits: 2^-17). Whatever the weights are they add up to 1, so that it is never off by more than twice the largest value that it sees (2^-7 for roundings).
+    off = 2 * (2.0 ** -8 if dtype == BF16 else 2.0 ** -17) * size
+    most = torch.stack([vv[:p + 1].abs().amax(0) for p in range(L - n, L)]).repeat_interleave(H // G, 1)
+    tol = tolerance(ref, 0.0 * size, mag, None, dtype) + torch.where(off < 40, mag * torch.expm1(off.clamp(max=40)), math.inf).minimum(2 * (1 + 2.0 ** -7) * most)
+    assert ((out.cpu().double().view(n, H, hd) - ref).abs() <= tol).all()
+    one = torch.empty(n, H * hd, dtype=dtype, device=DEV)
+    scratch = kernels.kv4_scratch(n, H, G, hd, DEV)
+    kernels.attn_decode_kv4(q.to(DEV), one, cache.to(DEV), tables.expand(n, -1).contiguous(), torch.arange(L - n, L, dtype=torch.int32, device=DEV),
+                            H, G, hd, hd ** -0.5, scratch=scratch)
+    assert ((one.cpu().double().view(n, H, hd) - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("what", ["portions", "few rows", "single tokens"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_same_call_gives_the_same_bits(what, dtype):
+    from vllm_oxide_b200 import kernels
+    H, G, hd, page = 24, 8, 128, 16
+    lens = [2600, 40, 3000] if what != "portions" else [700, 40, 900]
+    cache, tables, _, _ = paged(lens, G, hd, page, 5)
+    new = {"portions": [500, 40, 300], "few rows": [5, 1, 3], "single tokens": [1, 1, 1]}[what]
+    starts = torch.tensor([0, new[0], new[0] + new[1], sum(new)], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([a - b for a, b in zip(lens, new)], dtype=torch.int32, device=DEV)
+    q = torch.randn(sum(new), H * hd, generator=gen(6)).to(dtype).to(DEV)
+    scratch = kernels.kv4_scratch(3, H, G, hd, DEV)
+    first = None
+    for _ in range(20):
+        out = torch.full_like(q, 5.0)
+        if what == "single tokens":
+            kernels.attn_decode_kv4(q, out, cache, tables, ctx, H, G, hd, hd ** -0.5, scratch=scratch)
+        else:
+            kernels.attn_prefill_kv4(q, out, cache, tables, starts, ctx, 3, max(new), H, G, hd, hd ** -0.5)
+        first = out if first is None else first
+        assert torch.equal(out, first)

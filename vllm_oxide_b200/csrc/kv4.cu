@@ -748,8 +748,11 @@ int launch_portions(const void* q, long long q_stride, void* out, long long out_
     // an SM, 324 with two), more split what two already keep busy (600 tokens, a window of 100: 77 us unsplit, 162 split)
     const long long sees = min((long long)b.max_pages * b.page_size, b.window ? (long long)b.window + 16 * R : 0x7fffffffLL);
     const int parts = key_parts(tiles * b.G * S, 296, sees / (MIN_TILES * KEYS));
-    return launch_clusters(kv4_attend_kernel<T, DP, R>, dim3((unsigned)(tiles * parts), b.G, S), parts, dim3(FLEX_THREADS), flex_smem<DP, R>(), stream,
-                           (const T*)q, q_stride, (T*)out, out_stride, cache, b);
+    const dim3 grid((unsigned)(tiles * parts), b.G, S);
+    if (parts == 1)
+        return vob_launch(kv4_attend_kernel<T, DP, R>, grid, dim3(FLEX_THREADS), flex_smem<DP, R>(), stream, (const T*)q, q_stride, (T*)out, out_stride, cache, b);
+    return launch_clusters(kv4_attend_kernel<T, DP, R>, grid, parts, dim3(FLEX_THREADS), flex_smem<DP, R>(), stream, (const T*)q, q_stride, (T*)out,
+                           out_stride, cache, b);
 }
 
 template <typename T, int DP>

@@ -62,6 +62,13 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
     return x;
 }
+__device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
+    uint32_t at;
+    float4 x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+    return x;
+}
 // The weight of a part of a row's keys whose maximum (base 2) is `mine`: a part without keys has nothing to weigh (its sums are 0); one whose keys all
 // gave NaN has no maximum either, and stays NaN.
 __device__ __forceinline__ float part_weight(float mine, float all) { return mine == -INFINITY ? 1.f : exp2f(mine - all); }
@@ -71,6 +78,21 @@ static inline int key_parts(long long blocks, long long wanted, long long most) 
     int n = 1;
     while (n < 8 && blocks * n < wanted && 2 * n <= most) n *= 2;
     return n;
+}
+// Clusters of `parts` blocks that the current device runs at once.
+template <typename... P>
+static inline cudaError_t cluster_room(void (*kernel)(P...), int parts, dim3 block, size_t smem, int* clusters) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(parts * 148);
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg);
 }
 template <typename... P, typename... A>
 static inline int launch_clusters(void (*kernel)(P...), dim3 grid, int parts, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {

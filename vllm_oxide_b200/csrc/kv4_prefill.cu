@@ -28,6 +28,7 @@
 #include "kv4.cuh"
 VOB_PDL_SWITCH(kv4_prefill)
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "sm100.cuh"
 
 namespace {
@@ -35,6 +36,7 @@ using namespace vob_kv4;
 using namespace vob_sm100;
 
 constexpr int BM = 128, BN = 128, BS = 64;            // rows of a row tile, keys of a key tile, keys of a softmax step
+constexpr int MIN_TILES = 4;                          // key tiles that a block of a cluster has at least
 // Five warpgroups: softmax of the row tiles (2), codes to numbers of K and of V, issue of products (two threads). The registers that a block of 640
 // threads is launched with, 96 each, are shared out anew.
 constexpr int NTHREADS = 640;
@@ -107,13 +109,14 @@ __device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_
 
 template <int HD> constexpr size_t smem_bytes() { return 1024 + (size_t)(2 + 2 + 2) * (HD / 64) * SPAN + 512; }
 
-template <int HD>
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1)
 kv4_prefill_kernel(const Args a) {
     constexpr int NS = HD / 64;                                        // spans of 64 numbers
     constexpr int TILE = NS * SPAN;                                    // bytes of 128 rows of an operand
     pdl_launch_dependents();
-    const int group = a.H / a.G, kvh = blockIdx.x, seq = blockIdx.y;
+    const int parts = SPLIT ? (int)cluster_blocks() : 1, rank = SPLIT ? (int)cluster_rank() : 0;      // blocks that share the rows' keys
+    const int group = a.H / a.G, kvh = blockIdx.x / parts, seq = blockIdx.y;
     const int row0 = a.seq_starts[seq];
     const int total_rows = (a.seq_starts[seq + 1] - row0) * group;
     const int tile_rows = BM / group * group;                          // whole tokens only
@@ -144,7 +147,7 @@ kv4_prefill_kernel(const Args a) {
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // steps of 64 keys [from[t], to[t]) of each row tile, beginning with a key tile
+    // steps of 64 keys [from[t], to[t]) of each row tile that the block takes, beginning with a key tile
     int from[2], to[2], hi = 0, lo = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -158,8 +161,21 @@ kv4_prefill_kernel(const Args a) {
             lo = min(lo, l);
         }
     }
-    const int u0 = from[0], u1 = max(to[0], to[1]);                    // the first row tile has rows, and sees the earliest keys
-    const int j0 = u0 / 2, j1 = (u1 + 1) / 2;                          // key tiles
+    // key tiles [j0, j1) of the cluster (the first row tile has rows, and sees the earliest keys), and of the block
+    int j0 = from[0] / 2, j1 = (max(to[0], to[1]) + 1) / 2;
+    int used = 1;
+    if constexpr (SPLIT) {
+        const int share = max(MIN_TILES, (j1 - j0 + parts - 1) / parts);
+        used = (j1 - j0 + share - 1) / share;
+        if (used == 1 && rank) return;
+        j0 += rank * share;
+        j1 = max(j0, min(j1, j0 + share));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            from[t] = max(from[t], 2 * j0);
+            to[t] = min(to[t], 2 * j1);                                // (not behind `from`: the row tile has no step)
+        }
+    }
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -259,6 +275,7 @@ kv4_prefill_kernel(const Args a) {
             for (int j = j_to; j < j1 && ok; ++j) skip(j);
         }
         __syncwarp();
+        if (SPLIT && used > 1) { cluster_sync(); cluster_sync(); }                 // see the rows
     } else if (warp >= 8) {
         // ------------------------------------------------------------------ codes to numbers: K (warps 8 to 11), V (12 to 15)
         regs_down<REGS_CODES>();
@@ -329,6 +346,8 @@ kv4_prefill_kernel(const Args a) {
             load(j + 1, next);                                            // a tile ahead (behind the fence, which would wait for it)
             next = page_of(j + 2);
         }
+        __syncwarp();
+        if (SPLIT && used > 1) { cluster_sync(); cluster_sync(); }
     } else {
         // ------------------------------------------------------------------ softmax rows
         regs_up<REGS_ROWS>();
@@ -406,13 +425,15 @@ kv4_prefill_kernel(const Args a) {
             // P = 2^(score - m_ref + V's exponent) over the scores, and their sums. m_ref is some maximum of earlier steps: as long as no row's sum passes
             // 2^10 it may stay, since P, the sums and O are floating-point numbers relative to it.
             float sum_a, sum_b;
-            auto half = [&](const uint32_t (&v)[32], float sc, float shift, uint32_t to_column) {
-                const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(shift - m_ref, shift - m_ref);
+            // Behind a move a score is rounded before the reference is taken off it, as the reference was: the largest gives 1 however large scores are.
+            auto half = [&](auto moved, const uint32_t (&v)[32], float sc, float shift, uint32_t to_column) {
+                const float2 sc2 = make_float2(sc, sc), nm2 = decltype(moved)::value ? make_float2(shift, shift) : make_float2(shift - m_ref, shift - m_ref);
                 float2 acc = make_float2(0.f, 0.f);
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
+                    float2 x = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2);
+                    if constexpr (decltype(moved)::value) x = __fadd2_rn(x, make_float2(-m_ref, -m_ref));
                     const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                     acc = __fadd2_rn(acc, p);
                     pk[i >> 1] = pack_half(p.x, p.y);
@@ -420,13 +441,13 @@ kv4_prefill_kernel(const Args a) {
                 tmem_st16(tS + to_column, pk);                            // over scores that are in registers
                 return acc.x + acc.y;
             };
-            auto weigh = [&]() {
-                sum_a = half(va, sc_a, ev.x, 0);
-                sum_b = half(vb, sc_b, ev.y, 16);
+            auto weigh = [&](auto moved) {
+                sum_a = half(moved, va, sc_a, ev.x, 0);
+                sum_b = half(moved, vb, sc_b, ev.y, 16);
             };
             bool move = n == 0;
             if (!move) {
-                weigh();
+                weigh(std::false_type());
                 move = __any_sync(0xffffffffu, !(sum_a + sum_b <= 1024.f));
             }
             if (move) {
@@ -456,15 +477,21 @@ kv4_prefill_kernel(const Args a) {
                         tmem_st16(tO + c, v);
                     }
                 }
-                weigh();
+                weigh(std::true_type());
             }
             tmem_wait_st();
             tcgen05_fence_before();
             mbar_arrive(p_ready + 2 * t + b);
             l = fmaf(sum_a, v_inv.x, fmaf(sum_b, v_inv.y, l));
         }
-        if (ok && t_to > t_from && wait_all(o_done + t, 0, 50)) {
-            tcgen05_fence_after();
+        const bool have = ok && t_to > t_from && wait_all(o_done + t, 0, 50);       // O is there
+        tcgen05_fence_after();
+        // columns hold numbers 0 4 1 5 2 6 3 7
+        auto store8 = [&](__nv_bfloat16* to, const float* v, float f) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(v[0] * f, v[2] * f), pack_bf16(v[4] * f, v[6] * f), pack_bf16(v[1] * f, v[3] * f),
+                                                       pack_bf16(v[5] * f, v[7] * f));
+        };
+        if (used == 1 && have) {
             const float inv = nan_row ? NAN : l == 0.f ? 0.f : 1.f / l;
             __nv_bfloat16* dst = a.out + at * a.out_stride + (size_t)head * a.hd;
 #pragma unroll
@@ -473,18 +500,48 @@ kv4_prefill_kernel(const Args a) {
                 tmem_ld16(tO + c, v);
                 tmem_wait_ld();
                 if (valid && c < a.hd) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 8) {
-                        // columns hold numbers 0 4 1 5 2 6 3 7
-                        uint4 x;
-                        x.x = pack_bf16(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 2]) * inv);
-                        x.y = pack_bf16(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 6]) * inv);
-                        x.z = pack_bf16(__uint_as_float(v[e + 1]) * inv, __uint_as_float(v[e + 3]) * inv);
-                        x.w = pack_bf16(__uint_as_float(v[e + 5]) * inv, __uint_as_float(v[e + 7]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c + e) = x;
-                    }
+                    store8(dst + c, reinterpret_cast<const float*>(v), inv);
+                    store8(dst + c + 8, reinterpret_cast<const float*>(v) + 8, inv);
                 }
             }
+        } else if (SPLIT && used > 1) {
+            // the block's sums, where its tiles were, for the others: both row tiles' products have read them
+            constexpr int LD = HD + 4;
+            float* sO = reinterpret_cast<float*>(base);                  // [256][LD]
+            float* sM = sO + 2 * BM * LD;                                // [256] what O and l are relative to
+            float* sL = sM + 2 * BM;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            float* mine = sO + (t * BM + r) * LD;
+#pragma unroll
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t v[16] = {};
+                if (have) {
+                    tmem_ld16(tO + c, v);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(mine + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
+            sM[t * BM + r] = have ? m_ref : -INFINITY;
+            sL[t * BM + r] = nan_row ? NAN : have ? l : 0.f;
+            cluster_sync();
+            const int each = 2 * BM / parts;                             // rows that a block joins, 8 numbers a thread at a time
+            for (int i = threadIdx.x; i < each * (HD / 8); i += 2 * BM) {
+                const int row = rank * each + i / (HD / 8), c = i % (HD / 8) * 8;
+                const int in_tile = row % BM, row_at = first_row + row / BM * tile_rows + in_tile;
+                if (in_tile >= tile_rows || row_at >= total_rows || c >= a.hd) continue;
+                float all = -INFINITY, sum = 0.f, v[8] = {};
+                for (int p = 0; p < used; ++p) all = fmaxf(all, ld_cluster(sM + row, p));
+                for (int p = 0; p < used; ++p) {
+                    const float f = part_weight(ld_cluster(sM + row, p), all);
+                    const float4 lo4 = ld_cluster4(sO + row * LD + c, p), hi4 = ld_cluster4(sO + row * LD + c + 4, p);
+                    sum = fmaf(f, ld_cluster(sL + row, p), sum);
+                    v[0] = fmaf(f, lo4.x, v[0]); v[1] = fmaf(f, lo4.y, v[1]); v[2] = fmaf(f, lo4.z, v[2]); v[3] = fmaf(f, lo4.w, v[3]);
+                    v[4] = fmaf(f, hi4.x, v[4]); v[5] = fmaf(f, hi4.y, v[5]); v[6] = fmaf(f, hi4.z, v[6]); v[7] = fmaf(f, hi4.w, v[7]);
+                }
+                store8(a.out + (row0 + row_at / group) * a.out_stride + (size_t)(kvh * group + row_at % group) * a.hd + c, v, sum == 0.f ? 0.f : 1.f / sum);
+            }
+            cluster_sync();                                              // no block leaves while others read from it
         }
         tcgen05_fence_before();
     }
@@ -497,15 +554,29 @@ kv4_prefill_kernel(const Args a) {
 
 template <int HD> int launch(const Args& a, int S, long long row_tiles, cudaStream_t stream) {
     static char done[64] = {};
+    static int room[64][3] = {};                                         // clusters of 2, 4, 8 that the device runs at once
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
+    constexpr int smem = (int)smem_bytes<HD>();
+    const dim3 block(NTHREADS);
     if (dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(kv4_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<HD>());
-        if (e != cudaSuccess) return (int)e;
+        if ((e = cudaFuncSetAttribute(kv4_prefill_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return (int)e;
+        if ((e = cudaFuncSetAttribute(kv4_prefill_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return (int)e;
+        for (int i = 0; i < 3; ++i)
+            if ((e = cluster_room(kv4_prefill_kernel<HD, true>, 2 << i, block, smem, room[dev & 63] + i)) != cudaSuccess) return (int)e;
         if (dev < 64) done[dev] = 1;
     }
-    return vob_launch(kv4_prefill_kernel<HD>, dim3(a.G, S, (unsigned)row_tiles), dim3(NTHREADS), smem_bytes<HD>(), stream, a);
+    // Blocks that share keys where there are few: as many as find room at once, one on an SM. (A cluster stays within a part of the GPU, and has fewer SMs to
+    // choose from the larger it is: 74 of 2, 33 of 4 or 15 of 8 fit. 128 tokens behind 4,000 at 32/8 heads of 128, 16 blocks' worth of rows: 78.6 us unsplit,
+    // 39.6 by 4, 61.6 by 8; 16 tokens behind 8,000, 8 blocks' worth: 105, 40.1, 28.1.) Several requests count half of the longest's rows beyond one.
+    const long long sees = min((long long)a.max_pages * a.page_size, a.window ? (long long)a.window + 2 * BM : 0x7fffffffLL);
+    int parts = 1;
+    for (int i = 0; i < 3; ++i)
+        if (row_tiles * a.G * (S + 1) / 2 <= room[dev & 63][i] && (2 << i) * MIN_TILES * BN <= sees) parts = 2 << i;
+    const dim3 grid(a.G * parts, S, (unsigned)row_tiles);
+    if (parts == 1) return vob_launch(kv4_prefill_kernel<HD, false>, grid, block, smem, stream, a);
+    return launch_clusters(kv4_prefill_kernel<HD, true>, grid, parts, block, smem, stream, a);
 }
 
 }  // namespace
