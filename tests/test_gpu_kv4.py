@@ -418,3 +418,78 @@ def test_the_same_call_gives_the_same_bits(what, dtype):
             kernels.attn_prefill_kv4(q, out, cache, tables, starts, ctx, 3, max(new), H, G, hd, hd ** -0.5)
         first = out if first is None else first
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_captured_step_follows_its_inputs(dtype):
+    """append, attention of single tokens and of portions in one graph, replayed at other positions, slots and lengths."""
+    from vllm_oxide_b200 import kernels
+    H, G, hd, page, S, n = 8, 2, 64, 16, 3, 20
+    cache, tables, _, _ = paged([2500] * S, G, hd, page, 11)
+    f = freq(hd).to(DEV)
+    x = torch.randn(S + n, (H + 2 * G) * hd, generator=gen(12)).to(dtype).to(DEV)
+    ints = torch.zeros(4, S + n, dtype=torch.int32, device=DEV)
+    positions, slots, starts, contexts = ints
+    scratch = kernels.kv4_scratch(S, H, G, hd, DEV)
+    out = torch.empty(S + n, H * hd, dtype=dtype, device=DEV)
+    q_out = torch.empty_like(out)
+
+    def step():
+        kernels.kv4_append(x[:, :H * hd], x[:, H * hd:(H + G) * hd], x[:, (H + G) * hd:], positions, slots, f, cache, H, G, hd, q_out=q_out)
+        kernels.attn_decode_kv4(q_out[:S], out[:S], cache, tables, positions, H, G, hd, hd ** -0.5, scratch=scratch)
+        kernels.attn_prefill_kv4(q_out, out, cache, tables[1:2], starts, contexts, 1, n, H, G, hd, hd ** -0.5)
+
+    def place(lens, context):
+        pos = torch.tensor([m - 1 for m in lens] + list(range(context, context + n)), dtype=torch.int32)
+        rows = torch.tensor(list(range(S)) + [1] * n)
+        positions.copy_(pos)
+        slots.copy_(tables.cpu()[rows, pos.long() // page] * page + pos % page)
+        starts[:2] = torch.tensor([S, S + n], dtype=torch.int32)
+        contexts[:1] = context
+
+    place([5, 900, 40], 300)
+    step()
+    torch.cuda.synchronize()
+    before = cache.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for lens, context in (([2400, 17, 600], 1900), ([1, 2, 3], 2), ([700, 2100, 2500], 100)):            # (a token of request 1 and its portion never at one position: one slot a token)
+        place(lens, context)
+        cache.copy_(before)
+        graph.replay()
+        got, kept = out.clone(), cache.clone()
+        cache.copy_(before)
+        out.zero_()
+        step()
+        assert torch.equal(got, out) and torch.equal(kept, cache) and not got[:1].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_two_streams_at_once(dtype):
+    """Each with scratch of its own; the kernels share nothing else."""
+    from vllm_oxide_b200 import kernels
+    H, G, hd, page = 24, 8, 128, 16
+    cache, tables, _, _ = paged([3000, 700], G, hd, page, 21)
+    q = torch.randn(40, H * hd, generator=gen(22)).to(dtype).to(DEV)
+    pos = torch.tensor([2999, 500], dtype=torch.int32, device=DEV)
+    starts, ctx = torch.tensor([0, 30, 40], dtype=torch.int32, device=DEV), torch.tensor([2970, 600], dtype=torch.int32, device=DEV)
+
+    def both(scratch, one, many):
+        kernels.attn_decode_kv4(q[:2], one, cache, tables, pos, H, G, hd, hd ** -0.5, scratch=scratch)
+        kernels.attn_prefill_kv4(q, many, cache, tables, starts, ctx, 2, 30, H, G, hd, hd ** -0.5)
+
+    want = [torch.empty(2, H * hd, dtype=dtype, device=DEV), torch.empty_like(q)]
+    both(kernels.kv4_scratch(2, H, G, hd, DEV), *want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    scratches = [kernels.kv4_scratch(2, H, G, hd, DEV) for _ in streams]
+    outs = [[[torch.empty_like(w) for w in want] for _ in range(20)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                both(scratches[s], *outs[s][i])
+    torch.cuda.synchronize()
+    for per_stream in outs:
+        for got in per_stream:
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
