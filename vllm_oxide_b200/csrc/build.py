@@ -2,7 +2,7 @@
 
 Each `.cu` file under this folder is a module with a plain C interface (no torch headers,
 so a file compiles in seconds); each `.cpp` under `runtime/` builds into one pybind11
-module. A library is compiled at its first use for sm_100a, kept beside the sources in
+module (`kv4_calls.cpp` includes torch's headers: it reads tensors). A library is compiled at its first use for sm_100a, kept beside the sources in
 `_build/`, and rebuilt when its sources or flags change. There is no fallback: if a
 library cannot be built or loaded, the caller gets a `KernelError`.
 """
@@ -145,11 +145,13 @@ def runtime_module():
         if "runtime" in _loaded:
             return _loaded["runtime"]
         import pybind11
+        import torch
+        thome = os.path.dirname(torch.__file__)
         rdir = os.path.join(_HERE, "runtime")
         srcs = sorted(os.path.join(rdir, f) for f in os.listdir(rdir) if f.endswith(".cpp"))
         hdrs = sorted(os.path.join(rdir, f) for f in os.listdir(rdir) if f.endswith((".h", ".hpp")))
         hdrs += [f for f in _headers() if f.endswith(".h")]        # what host and kernels share
-        tag = _digest(srcs + hdrs, _CXX_FLAGS + [sys.version])
+        tag = _digest(srcs + hdrs, _CXX_FLAGS + [sys.version, torch.__version__])
         bdir = _build_dir()
         so = os.path.join(bdir, f"vob200_runtime_{tag}.so")
         if not os.path.exists(so):
@@ -165,8 +167,10 @@ def runtime_module():
             print("[vllm_oxide_b200] compiling the host runtime (C++) ...", file=sys.stderr, flush=True)
             tmp = so + f".{os.getpid()}.tmp"
             _run([cxx] + _CXX_FLAGS + [f"-DVOB_MODULE_NAME=vob200_runtime_{tag}",
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                   "-I", pybind11.get_include(), "-I", sysconfig.get_paths()["include"], "-I", rdir, "-I", _HERE,
-                  "-o", tmp] + srcs, "runtime")
+                  "-isystem", os.path.join(thome, "include"), "-o", tmp] + srcs
+                 + ["-L" + os.path.join(thome, "lib"), "-lstdc++", "-ltorch_python", "-ltorch_cpu", "-lc10"], "runtime")
             os.replace(tmp, so)
         spec = importlib.util.spec_from_file_location(f"vob200_runtime_{tag}", so)
         try:

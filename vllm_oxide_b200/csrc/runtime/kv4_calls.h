@@ -1,335 +1,7 @@
-// The host side of the 4-bit cache's operators: every check of a call and the call of the kernel library's entry point.
-//
-// The kernels of a decode step take 3 to 10 us, and the same checks in Python, some fifty properties of eight tensors, took 9 of a call's 12 us. Here a
-// tensor's properties are read once each through the CPython API, and the entry point is called directly: some 5 us, the launch included.
-// Shapes, types and strides are checked before the device, so that a call that does not fit is refused wherever its tensors are; a call that fits
-// and whose tensors are on no CUDA device is a KernelError (there is no CPU path). A call returns the entry point's status, or -1 where there was nothing
-// to launch.
+// The calls of the 4-bit cache's operators (kv4_calls.cpp), as functions of the runtime module.
 #pragma once
 #include <Python.h>
-#include <cstdarg>
-#include <cstdint>
-#include <cstdio>
 
 namespace vob_calls {
-
-struct Known {
-    PyObject *shape_error = nullptr, *kernel_error = nullptr;
-    PyObject *f32 = nullptr, *bf16 = nullptr, *u8 = nullptr, *i32 = nullptr;     // torch dtypes
-    PyObject *get_device = nullptr, *raw_stream = nullptr;                       // torch._C._cuda_getDevice, _cuda_getCurrentRawStream
-    PyObject *n_shape, *n_stride, *n_dtype, *n_device, *n_ptr;                   // interned names
-};
-inline Known& known() {
-    static Known k;
-    return k;
+PyMethodDef* methods();
 }
-
-// Raises ShapeError(op, message); false for the caller to hand on.
-inline bool refuse(const char* op, const char* format, ...) {
-    char text[512];
-    va_list ap;
-    va_start(ap, format);
-    vsnprintf(text, sizeof text, format, ap);
-    va_end(ap);
-    PyObject* e = PyObject_CallFunction(known().shape_error, "ss", op, text);
-    if (e) {
-        PyErr_SetObject(known().shape_error, e);
-        Py_DECREF(e);
-    }
-    return false;
-}
-
-struct Tensor {
-    const char* name = "";
-    bool there = false;
-    int dims = 0, device = -1;
-    int64_t size[4] = {0, 0, 0, 0}, stride[4] = {0, 0, 0, 0};
-    PyObject* dtype = nullptr;              // borrowed: dtypes live as long as torch does
-    void* ptr = nullptr;
-
-    // Reads the properties of `t`; None where `optional`.
-    bool read(PyObject* t, const char* op, const char* what, bool optional = false) {
-        name = what;
-        if (t == Py_None && optional) return true;
-        Known& k = known();
-        PyObject* v = PyObject_GetAttr(t, k.n_shape);
-        if (!v || !PyTuple_Check(v)) {
-            Py_XDECREF(v);
-            PyErr_Clear();
-            return refuse(op, "%s must be a tensor", what);
-        }
-        dims = (int)PyTuple_GET_SIZE(v);
-        if (dims <= 4)
-            for (int i = 0; i < dims; ++i) size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(v, i));
-        Py_DECREF(v);
-        if (dims > 4) return refuse(op, "%s has %d dimensions", what, dims);
-        v = PyObject_CallMethodNoArgs(t, k.n_stride);
-        if (!v) return false;
-        for (int i = 0; i < dims; ++i) stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(v, i));
-        Py_DECREF(v);
-        dtype = PyObject_GetAttr(t, k.n_dtype);
-        if (!dtype) return false;
-        Py_DECREF(dtype);
-        v = PyObject_CallMethodNoArgs(t, k.n_device);
-        if (!v) return false;
-        device = (int)PyLong_AsLong(v);
-        Py_DECREF(v);
-        v = PyObject_CallMethodNoArgs(t, k.n_ptr);
-        if (!v) return false;
-        ptr = PyLong_AsVoidPtr(v);
-        Py_DECREF(v);
-        there = true;
-        return !PyErr_Occurred();
-    }
-    bool contiguous() const {
-        int64_t n = 1;
-        for (int i = dims - 1; i >= 0; --i) {
-            if (size[i] != 1 && stride[i] != n) return false;
-            n *= size[i];
-        }
-        return true;
-    }
-    int code() const { return dtype == known().f32 ? 0 : dtype == known().bf16 ? 1 : -1; }
-
-    // [rows, cols] of the type of `like` with unit inner stride; rows < 0: any number
-    bool rows(const char* op, int64_t n, int64_t cols, const Tensor& like) const {
-        if (like.code() < 0) return refuse(op, "%s: only float32 and bfloat16 are supported", like.name);
-        if (dims != 2 || (n >= 0 && size[0] != n) || size[1] != cols || dtype != like.dtype || (stride[1] != 1 && cols > 1))
-            return refuse(op, "%s must be %s [%lld, %lld] with unit inner stride, got %d dimensions [%lld, %lld] strides [%lld, %lld]%s", name,
-                          like.code() ? "bfloat16" : "float32", (long long)(n >= 0 ? n : size[0]), (long long)cols, dims, (long long)size[0],
-                          (long long)size[1], (long long)stride[0], (long long)stride[1], dtype != like.dtype ? " of another type" : "");
-        return true;
-    }
-    bool ints(const char* op, int64_t n) const {
-        if (dtype != known().i32 || dims != 1 || size[0] < n || !contiguous())
-            return refuse(op, "%s must be a contiguous int32 vector of at least %lld, got %d dimensions [%lld]%s", name, (long long)n, dims,
-                          (long long)size[0], dtype != known().i32 ? " of another type" : "");
-        return true;
-    }
-    bool aligned(int bytes, int elements) const { return (uintptr_t)ptr % bytes == 0 && stride[0] % elements == 0; }
-};
-
-// One layer's cache (csrc/kv4.cuh).
-inline bool check_cache(const char* op, const Tensor& c, long long heads, long long kv_heads, long long hd) {
-    const long long width = 32 * ((hd + 31) / 32) + 8;
-    if (c.dtype != known().u8 || c.dims != 4 || c.size[1] != kv_heads || c.size[3] != width || !c.contiguous() || c.size[0] < 1)
-        return refuse(op, "the cache must be contiguous uint8 [pages, %lld, page_size, %lld], got %d dimensions [%lld, %lld, %lld, %lld]%s", kv_heads, width, c.dims,
-                      (long long)c.size[0], (long long)c.size[1], (long long)c.size[2], (long long)c.size[3], c.dtype != known().u8 ? " of another type" : "");
-    if (c.size[0] * c.size[2] > 0x7fffffffLL) return refuse(op, "%lld pages of %lld tokens are beyond 2^31 - 1 slots", (long long)c.size[0], (long long)c.size[2]);
-    if ((uintptr_t)c.ptr % 16) return refuse(op, "the cache must start on a 16-byte boundary");
-    if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || hd <= 0 || hd > 256 || hd % 16 || c.size[2] <= 0 || c.size[2] % 8)
-        return refuse(op, "sizes not supported: heads %lld/%lld, head_dim %lld (multiples of 16 up to 256), page %lld (multiples of 8)", heads, kv_heads, hd,
-                      (long long)c.size[2]);
-    return true;
-}
-
-// All tensors on the current CUDA device; its current stream.
-inline bool find_stream(const char* op, const Tensor* const* tensors, int n, void** stream) {
-    Known& k = known();
-    for (int i = 0; i < n; ++i)
-        if (tensors[i]->there && tensors[i]->device < 0) {
-            PyErr_Format(k.kernel_error, "%s: %s is not on a CUDA device; the kernels run there only (there is no CPU path)", op, tensors[i]->name);
-            return false;
-        }
-    PyObject* v = PyObject_CallNoArgs(k.get_device);
-    if (!v) return false;
-    const int device = (int)PyLong_AsLong(v);
-    for (int i = 0; i < n; ++i)
-        if (tensors[i]->there && tensors[i]->device != device) {
-            Py_DECREF(v);
-            return refuse(op, "%s is on cuda:%d, the current device is cuda:%d: launches go to its stream", tensors[i]->name, tensors[i]->device, device);
-        }
-    PyObject* s = PyObject_CallOneArg(k.raw_stream, v);
-    Py_DECREF(v);
-    if (!s) return false;
-    *stream = PyLong_AsVoidPtr(s);
-    Py_DECREF(s);
-    return !PyErr_Occurred();
-}
-
-inline bool whole(PyObject* o, long long* v) {
-    *v = PyLong_AsLongLong(o);
-    return !(*v == -1 && PyErr_Occurred());
-}
-inline bool address(PyObject* o, void** v) {
-    *v = PyLong_AsVoidPtr(o);
-    return !(!*v && PyErr_Occurred());
-}
-
-typedef int (*AppendFn)(const void*, long long, void*, long long, const void*, long long, const void*, long long, const int*, const int*, const float*, void*,
-                        long long, int, int, int, int, int, int, void*);
-typedef int (*ReadFn)(const void*, long long, const int*, void*, long long, void*, long long, int, int, int, int, int, void*);
-typedef int (*AttendFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, const int*, const int*, int, int, int,
-                        int, int, int, float, int, int, int, float*, long long, int*, long long, void*);
-typedef int (*DecodeFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, int, int, int, int, int, float, int,
-                        float*, long long, int*, long long, int, int*, void*);
-typedef int (*PrefillFn)(const void*, long long, void*, long long, const void*, long long, const int*, int, const int*, const int*, int, int, int, int, int,
-                         int, float, int, int*, void*);
-
-#define VOB_ARGS(n)                                                                   \
-    if (count != n) {                                                                 \
-        PyErr_Format(PyExc_TypeError, "%s: %zd arguments instead of %d", op, count, n); \
-        return nullptr;                                                               \
-    }
-
-// (entry, q, k, v, positions, slots, inv_freq, cache, heads, kv heads, head size, q_out) -> status
-inline PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    const char* op = "kv4_append";
-    VOB_ARGS(12)
-    void *entry, *stream;
-    long long H, G, hd;
-    Tensor q, k, v, pos, slots, freq, cache, out;
-    if (!address(a[0], &entry) || !whole(a[8], &H) || !whole(a[9], &G) || !whole(a[10], &hd)) return nullptr;
-    if (!q.read(a[1], op, "q") || !k.read(a[2], op, "k") || !v.read(a[3], op, "v") || !pos.read(a[4], op, "positions") ||
-        !slots.read(a[5], op, "slots", true) || !freq.read(a[6], op, "inv_freq", true) || !cache.read(a[7], op, "cache") || !out.read(a[11], op, "q_out", true))
-        return nullptr;
-    if (!check_cache(op, cache, H, G, hd) || !q.rows(op, -1, H * hd, q)) return nullptr;
-    const int64_t T = q.size[0];
-    if (!k.rows(op, T, G * hd, q) || !v.rows(op, T, G * hd, q) || (out.there && !out.rows(op, T, H * hd, q)) || !pos.ints(op, T) ||
-        (slots.there && !slots.ints(op, T)))
-        return nullptr;
-    if (freq.there && (freq.dtype != known().f32 || freq.dims != 1 || freq.size[0] != hd / 2 || !freq.contiguous())) {
-        refuse(op, "inv_freq must be contiguous float32 [%lld]", hd / 2);
-        return nullptr;
-    }
-    if (T > 0x7fffffffLL) { refuse(op, "%lld tokens", (long long)T); return nullptr; }
-    const Tensor* all[] = {&q, &k, &v, &pos, &slots, &freq, &cache, &out};
-    if (!find_stream(op, all, 8, &stream)) return nullptr;
-    if (T == 0) return PyLong_FromLong(-1);
-    const Tensor& to = out.there ? out : q;
-    return PyLong_FromLong(((AppendFn)entry)(q.ptr, q.stride[0], to.ptr, to.stride[0], k.ptr, k.stride[0], v.ptr, v.stride[0], (int*)pos.ptr, (int*)slots.ptr,
-                                             (float*)freq.ptr, cache.ptr, cache.size[0], q.code(), (int)T, (int)H, (int)G, (int)hd, (int)cache.size[2], stream));
-}
-
-// (entry, cache, slots, k_out, v_out, kv heads, head size) -> status
-inline PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    const char* op = "kv4_read";
-    VOB_ARGS(7)
-    void *entry, *stream;
-    long long G, hd;
-    Tensor cache, slots, k, v;
-    if (!address(a[0], &entry) || !whole(a[5], &G) || !whole(a[6], &hd)) return nullptr;
-    if (!cache.read(a[1], op, "cache") || !slots.read(a[2], op, "slots") || !k.read(a[3], op, "k_out") || !v.read(a[4], op, "v_out")) return nullptr;
-    if (!check_cache(op, cache, G, G, hd) || !k.rows(op, -1, G * hd, k) || !v.rows(op, k.size[0], G * hd, k) || !slots.ints(op, k.size[0])) return nullptr;
-    if (k.size[0] > 0x7fffffffLL) { refuse(op, "%lld tokens", (long long)k.size[0]); return nullptr; }
-    const Tensor* all[] = {&cache, &slots, &k, &v};
-    if (!find_stream(op, all, 4, &stream)) return nullptr;
-    if (k.size[0] == 0) return PyLong_FromLong(-1);
-    return PyLong_FromLong(((ReadFn)entry)(cache.ptr, cache.size[0], (int*)slots.ptr, k.ptr, k.stride[0], v.ptr, v.stride[0], k.code(), (int)k.size[0], (int)G,
-                                           (int)hd, (int)cache.size[2], stream));
-}
-
-// What both attention calls check of q, out, cache and block tables.
-inline bool check_attention(const char* op, const Tensor& q, const Tensor& out, const Tensor& cache, const Tensor& tables, long long seqs, long long H,
-                            long long G, long long hd, long long window) {
-    if (!check_cache(op, cache, H, G, hd) || !q.rows(op, -1, H * hd, q) || !out.rows(op, q.size[0], H * hd, q)) return false;
-    if (tables.dtype != known().i32 || tables.dims != 2 || !tables.contiguous() || tables.size[1] < 1 || tables.size[1] > 0x7fffffffLL)
-        return refuse(op, "block_tables must be contiguous int32 [S, max_pages]");
-    if (tables.size[0] < seqs) return refuse(op, "block_tables has %lld rows for %lld requests", (long long)tables.size[0], seqs);
-    if (window < 0 || window > 0x7fffffffLL) return refuse(op, "window %lld", window);
-    if (q.size[0] > 0x7fffffffLL) return refuse(op, "%lld rows", (long long)q.size[0]);
-    return true;
-}
-
-// (entry, entry in 32-bit arithmetic, q, out, cache, block_tables, positions, heads, kv heads, head size, scale, window, partials, arrived, the scratch's
-//  (requests, heads, kv heads, head size), SMs, error word) -> status
-inline PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    const char* op = "attn_decode_kv4";
-    VOB_ARGS(17)
-    void *entry, *general, *stream, *err;
-    long long H, G, hd, window, sms, made[4];
-    Tensor q, out, cache, tables, pos, partials, arrived;
-    const double scale = PyFloat_AsDouble(a[10]);
-    if (PyErr_Occurred() || !address(a[0], &entry) || !address(a[1], &general) || !whole(a[7], &H) || !whole(a[8], &G) || !whole(a[9], &hd) ||
-        !whole(a[11], &window) || !whole(a[15], &sms) || !address(a[16], &err))
-        return nullptr;
-    if (!PyTuple_Check(a[14]) || PyTuple_GET_SIZE(a[14]) != 4) { refuse(op, "scratch must come from kv4_scratch"); return nullptr; }
-    for (int i = 0; i < 4; ++i)
-        if (!whole(PyTuple_GET_ITEM(a[14], i), &made[i])) return nullptr;
-    if (!q.read(a[2], op, "q") || !out.read(a[3], op, "out") || !cache.read(a[4], op, "cache") || !tables.read(a[5], op, "block_tables") ||
-        !pos.read(a[6], op, "positions") || !partials.read(a[12], op, "partials") || !arrived.read(a[13], op, "arrived"))
-        return nullptr;
-    const int64_t S = q.size[0];
-    if (!check_attention(op, q, out, cache, tables, q.dims == 2 ? S : 0, H, G, hd, window) || !pos.ints(op, S)) return nullptr;
-    if (S > made[0] || H != made[1] || G != made[2] || hd != made[3]) {
-        refuse(op, "the scratch was made for %lld requests of (%lld, %lld, %lld) (heads, kv heads, head size), not for %lld of (%lld, %lld, %lld)", made[0],
-               made[1], made[2], made[3], (long long)S, H, G, hd);
-        return nullptr;
-    }
-    const Tensor* all[] = {&q, &out, &cache, &tables, &pos, &partials, &arrived};
-    if (!find_stream(op, all, 7, &stream)) return nullptr;
-    if (S == 0) return PyLong_FromLong(-1);
-    if (q.code() == 1 && q.aligned(16, 8) && out.aligned(4, 2))
-        return PyLong_FromLong(((DecodeFn)entry)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
-                                                 (int*)pos.ptr, (int)S, (int)H, (int)G, (int)hd, (int)cache.size[2], (float)scale, (int)window,
-                                                 (float*)partials.ptr, partials.size[0], (int*)arrived.ptr, arrived.size[0], (int)sms, (int*)err, stream));
-    // 32-bit arithmetic: the float32 engine, and rows that the tensor-core kernel cannot address. Blocks of 4 heads, eight an SM
-    const long long blocks = S * G * ((H / G + 3) / 4);
-    long long splits = 8 * sms / blocks;
-    splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
-    return PyLong_FromLong(((AttendFn)general)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
-                                               (int*)pos.ptr, nullptr, nullptr, (int)S, 1, (int)H, (int)G, (int)hd, (int)cache.size[2], (float)scale,
-                                               (int)window, q.code(), (int)splits, (float*)partials.ptr, partials.size[0], (int*)arrived.ptr, arrived.size[0], stream));
-}
-
-// (entry, entry in 32-bit arithmetic, q, out, cache, block_tables, seq_starts, context_lens, requests, longest portion, heads, kv heads, head size, scale,
-//  window, error word) -> status
-inline PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    const char* op = "attn_prefill_kv4";
-    VOB_ARGS(16)
-    void *entry, *general, *stream, *err;
-    long long S, longest, H, G, hd, window;
-    Tensor q, out, cache, tables, starts, contexts;
-    const double scale = PyFloat_AsDouble(a[13]);
-    if (PyErr_Occurred() || !address(a[0], &entry) || !address(a[1], &general) || !whole(a[8], &S) || !whole(a[9], &longest) || !whole(a[10], &H) ||
-        !whole(a[11], &G) || !whole(a[12], &hd) || !whole(a[14], &window) || !address(a[15], &err))
-        return nullptr;
-    if (!q.read(a[2], op, "q") || !out.read(a[3], op, "out") || !cache.read(a[4], op, "cache") || !tables.read(a[5], op, "block_tables") ||
-        !starts.read(a[6], op, "seq_starts") || !contexts.read(a[7], op, "context_lens"))
-        return nullptr;
-    if (S < 0 || S > 0x7ffffffe || longest < 0 || longest > 0x7fffffffLL) { refuse(op, "%lld requests, the longest of %lld tokens", S, longest); return nullptr; }
-    if (!check_attention(op, q, out, cache, tables, S, H, G, hd, window) || !starts.ints(op, S + 1) || !contexts.ints(op, S)) return nullptr;
-    const Tensor* all[] = {&q, &out, &cache, &tables, &starts, &contexts};
-    if (!find_stream(op, all, 6, &stream)) return nullptr;
-    if (S == 0 || longest == 0) return PyLong_FromLong(-1);
-    if (q.code() == 1 && hd <= 128 && H / G <= 128 && (float)scale > 0.f && q.aligned(16, 8) && out.aligned(16, 8))
-        return PyLong_FromLong(((PrefillFn)entry)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
-                                                  (int*)starts.ptr, (int*)contexts.ptr, (int)S, (int)longest, (int)H, (int)G, (int)hd, (int)cache.size[2],
-                                                  (float)scale, (int)window, (int*)err, stream));
-    // 32-bit arithmetic: the float32 engine, larger heads, and rows that the tensor-core kernel cannot address
-    return PyLong_FromLong(((AttendFn)general)(q.ptr, q.stride[0], out.ptr, out.stride[0], cache.ptr, cache.size[0], (int*)tables.ptr, (int)tables.size[1],
-                                               nullptr, (int*)starts.ptr, (int*)contexts.ptr, (int)S, (int)longest, (int)H, (int)G, (int)hd,
-                                               (int)cache.size[2], (float)scale, (int)window, q.code(), 1, nullptr, 0, nullptr, 0, stream));
-}
-
-// (ShapeError, KernelError, float32, bfloat16, uint8, int32, get_device, raw_stream): what the calls need to know of Python, once.
-inline PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    const char* op = "kv4_setup";
-    VOB_ARGS(8)
-    Known& k = known();
-    PyObject** to[] = {&k.shape_error, &k.kernel_error, &k.f32, &k.bf16, &k.u8, &k.i32, &k.get_device, &k.raw_stream};
-    for (int i = 0; i < 8; ++i) {
-        Py_INCREF(a[i]);
-        Py_XDECREF(*to[i]);
-        *to[i] = a[i];
-    }
-    k.n_shape = PyUnicode_InternFromString("shape");
-    k.n_stride = PyUnicode_InternFromString("stride");
-    k.n_dtype = PyUnicode_InternFromString("dtype");
-    k.n_device = PyUnicode_InternFromString("get_device");
-    k.n_ptr = PyUnicode_InternFromString("data_ptr");
-    Py_RETURN_NONE;
-}
-#undef VOB_ARGS
-
-inline PyMethodDef* methods() {
-    static PyMethodDef all[] = {{"kv4_setup", (PyCFunction)(void*)setup, METH_FASTCALL, nullptr},
-                                {"kv4_append", (PyCFunction)(void*)append, METH_FASTCALL, nullptr},
-                                {"kv4_read", (PyCFunction)(void*)read, METH_FASTCALL, nullptr},
-                                {"attn_decode_kv4", (PyCFunction)(void*)decode, METH_FASTCALL, nullptr},
-                                {"attn_prefill_kv4", (PyCFunction)(void*)prefill, METH_FASTCALL, nullptr},
-                                {nullptr, nullptr, 0, nullptr}};
-    return all;
-}
-
-}  // namespace vob_calls

@@ -2248,8 +2248,8 @@ def kv4_supported(num_heads: int, num_kv_heads: int, head_dim: int, page_size: i
             and page_size > 0 and page_size % 8 == 0)
 
 
-# The calls of this cache are made by the native runtime (csrc/runtime/kv4_calls.h): its checks of every shape, type, stride, device and alignment take
-# half a microsecond a tensor less than here, which is what such a call of a decode step is made of.
+# The calls of this cache are made by the native runtime (csrc/runtime/kv4_calls.cpp): its checks of every shape, type, stride, device and alignment take
+# a microsecond a tensor less than here, which is what such a call of a decode step is made of.
 _kv4_native = None
 
 
@@ -2259,8 +2259,7 @@ class _KV4Calls:
     def __init__(self):
         from .csrc.build import runtime_module
         rt = runtime_module()
-        rt.kv4_setup(ShapeError, KernelError, torch.float32, torch.bfloat16, torch.uint8, torch.int32,
-                     getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None))
+        rt.kv4_setup(ShapeError, KernelError, getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None))
         self.append, self.read, self.decode, self.prefill = rt.kv4_append, rt.kv4_read, rt.attn_decode_kv4, rt.attn_prefill_kv4
 
         def entry(module, name):
