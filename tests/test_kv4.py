@@ -123,3 +123,13 @@ def test_architectures_say_what_they_cache():
     from vllm_oxide_b200 import models  # noqa: F401
     from vllm_oxide_b200.config import architecture_for, known_architectures
     assert [a for a in known_architectures() if 4 in architecture_for({"architectures": [a]}).cache_bits] == ["LlamaForCausalLM"]
+
+
+@pytest.mark.parametrize("odd", [5, None, "q", torch.zeros(3, 128).to_sparse(), torch.zeros(1, 1, 1, 3, 128), torch.zeros(3, 128, dtype=torch.complex64),
+                                 torch.zeros((), dtype=torch.float32), torch.zeros(0)])
+def test_what_is_no_tensor_with_rows_is_refused(no_gpu, odd):
+    with pytest.raises(ShapeError):
+        kernels.kv4_append(**_append_args(q=odd))
+    with pytest.raises(ShapeError):
+        kernels.attn_prefill_kv4(**_attn_args(q=odd, seq_starts=torch.zeros(4, dtype=torch.int32), context_lens=torch.zeros(3, dtype=torch.int32),
+                                              num_seqs=3, max_new=1))

@@ -20,7 +20,8 @@ using namespace vob_kv4;
 // takes 2 tokens, four warps a token (where there are few, one token, and up to some blocks share it), so that what belongs to a token (its slot, the sines of a
 // lane's pairs) is looked up once. The loads of a warp are on their way together, before the sines are taken: with 32/8 heads of 128 it has 4 pairs of
 // queries and 2 of keys and values, 3 KB in flight.
-// Bound: memory (reads q, k, v once, writes q and 136 of 512 bytes per key and value at D = 128).
+// Least traffic: q, k, v read once, q and 136 of 512 bytes per key and value at D = 128 written. 2,048 tokens at 32/8 heads of 128, bfloat16: 18.9 us, 44 MB, 2.3
+// TB/s. Bound: latency. 16 warps an SM (120 registers a thread) use 47 % of the issue slots, and 3.5 waves of blocks leave the last one half empty.
 // ---------------------------------------------------------------------------------------------
 constexpr int APPEND_WARPS = 8;
 
@@ -335,7 +336,9 @@ template <int ZERO = 8> __device__ __forceinline__ float code_number(uint32_t w,
 // Single tokens. A block has 4 heads of one request and kv head, and `splits` blocks share the request's keys; each of its warps takes 32 keys at a time, by
 // itself: a lane a key for the scores, sum(q (n - 8)) s + (m + 8 s) sum(q) on the codes as they come from the cache, then two numbers a lane (NB times 64 numbers) for the
 // sums, the codes of the values going through shared memory. The warps' results meet at the end, the blocks' in the block that arrives last, in the
-// order of the keys. Bound: instructions (some 16 per key and 32 lanes for the scores, as many for the sums, at 4 heads of 64).
+// order of the keys. 6 requests of 90 to 1,501 tokens at 32/8 heads of 64, float32: 13.1 us. Bound: the latency of one tile (a
+// table entry, the codes, the join), as a block has one or two there; with more of them instructions (some 16 per key and 32 lanes for the
+// scores, as many for the sums, at 4 heads of 64).
 constexpr int SINGLE_ROWS = 4, SINGLE_WARPS = 4;
 
 template <typename T, int NB>
@@ -521,8 +524,8 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
 // Portions. One block: 16 R rows (token, head of the group) of one request and kv head, over KEYS keys at a time. Codes become numbers in shared memory once
 // per tile (fetched a tile ahead). A thread has R rows x 4 keys of the scores (16 threads share a row), the rows' maxima and sums and R rows x DP / 16
 // numbers of the sums in registers; the probabilities cross over within its warp. Where there are few rows a cluster of blocks shares their keys.
-// Bound: the FMA pipe at R = 4 (a tile's 64 keys x 4 rows take 2 x 4 x 64 FMAs a thread and 64 numbers, and 3/4 of the shared memory's
-// time), shared memory at R = 1, which is for requests of few rows.
+// Bound: shared memory (69 % of its cycles; the FMA pipe 48 %). 600 tokens behind 1,000 at 32/8 heads of 64, float32: 271 us, 24 TFLOP/s; tiles of 16 rows,
+// a key a thread, took 561. R = 1 is for requests of few rows. (Three blocks an SM instead of two: 318 us.)
 constexpr int KEYS = 64, FLEX_THREADS = 256, MIN_TILES = 2;            // tiles of keys that a block of a cluster has at least
 
 template <int DP, int R> constexpr size_t flex_smem() {

@@ -2346,8 +2346,9 @@ def attn_prefill_kv4(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, bl
     longest portion (a request's rows beyond it are not computed). `window` and what becomes NaN: as `attn_decode_kv4`. Rows that
     belong to no request are left as they are."""
     n = _kv4_native or _kv4()
+    err = _scratch_for(q.device).err.data_ptr() if isinstance(q, torch.Tensor) and q.is_cuda else 0            # (what is no such tensor is refused there)
     _kv4_done(n.prefill(n.prefill_entry, n.attend_entry, q, out, cache, block_tables, seq_starts, context_lens, num_seqs, max_new, num_heads, num_kv_heads,
-                        head_dim, scale, window, _scratch_for(q.device).err.data_ptr()), "attn_prefill_kv4")
+                        head_dim, scale, window, err), "attn_prefill_kv4")
 
 
 # ------------------------------------------------------------------------------------ sampling
