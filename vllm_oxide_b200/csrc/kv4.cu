@@ -336,10 +336,11 @@ template <int ZERO = 8> __device__ __forceinline__ float code_number(uint32_t w,
 // Single tokens. A block has 4 heads of one request and kv head, and `splits` blocks share the request's keys; each of its warps takes 32 keys at a time, by
 // itself: a lane a key for the scores, sum(q (n - 8)) s + (m + 8 s) sum(q) on the codes as they come from the cache, then two numbers a lane (NB times 64 numbers) for the
 // sums, the codes of the values going through shared memory. The warps' results meet at the end, the blocks' in the block that arrives last, in the
-// order of the keys. 6 requests of 90 to 1,501 tokens at 32/8 heads of 64, float32: 13.1 us. Bound: the latency of one tile (a
+// order of the keys. 6 requests of 90 to 1,501 tokens at 32/8 heads of 64, float32: 10.5 us (13.2 while each
+// thread took the parts' maxima and weights for itself). Bound: the latency of one tile (a
 // table entry, the codes, the join), as a block has one or two there; with more of them instructions (some 16 per key and 32 lanes for the
 // scores, as many for the sums, at 4 heads of 64).
-constexpr int SINGLE_ROWS = 4, SINGLE_WARPS = 4;
+constexpr int SINGLE_ROWS = 4, SINGLE_WARPS = 4, MAX_SPLITS = 64;
 
 template <typename T, int NB>
 __global__ void __launch_bounds__(32 * SINGLE_WARPS, 4)
@@ -351,6 +352,7 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
     __shared__ __align__(16) float4 sP[W][32];
     __shared__ __align__(16) unsigned char sV[W][32][32 * NB];
     __shared__ float sO[W][R][DP];
+    __shared__ float sF[R][MAX_SPLITS], sAll[R], sSum[R];  // weights of the parts that meet, of the warps or of the blocks
     __shared__ int is_last;
     pdl_launch_dependents();
     pdl_wait(35);
@@ -367,9 +369,11 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
     const int t_lo = lo / TILE, t_hi = (hi + TILE - 1) / TILE, share = (t_hi - t_lo + splits - 1) / splits;
     const int used = (t_hi - t_lo + share - 1) / share, t0 = t_lo + split * share, t1 = min(t_hi, t0 + share);
     if (t0 >= t1) return;
-    for (int i = threadIdx.x; i < R * DP; i += 32 * W) {
-        const int r = i / DP, d = i % DP;
-        sQ[r][d] = r < heads && d < hd ? ld_f(q + (size_t)seq * q_stride + (size_t)(head0 + r) * hd + d) * b.scale : 0.f;
+    const float scale = b.scale * 1.4426950408889634f;     // probabilities are powers of two
+#pragma unroll
+    for (int k = 0; k < R * DP / (32 * W); ++k) {
+        const int i = threadIdx.x + k * 32 * W, r = i / DP, d = i % DP;
+        sQ[r][d] = r < heads && d < hd ? ld_f(q + (size_t)seq * q_stride + (size_t)(head0 + r) * hd + d) * scale : 0.f;
     }
     __syncthreads();
     if (warp < R) {
@@ -408,14 +412,21 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
             }
         }
         float s[R] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = 0; c < C; ++c) {
-            uint4 kn = make_uint4(0, 0, 0, 0), vn = kn;
-            if (grp) {
-                kn = *reinterpret_cast<const uint4*>(grp + c * 128);
-                vn = *reinterpret_cast<const uint4*>(grp + (C + c) * 128);
+        uint4 kn[2 * NB], vn[2 * NB];                       // all on their way at once
+#pragma unroll
+        for (int c = 0; c < 2 * NB; ++c) {
+            kn[c] = vn[c] = make_uint4(0, 0, 0, 0);
+            if (grp && c < C) {
+                kn[c] = *reinterpret_cast<const uint4*>(grp + c * 128);
+                vn[c] = *reinterpret_cast<const uint4*>(grp + (C + c) * 128);
             }
-            *reinterpret_cast<uint4*>(&sV[warp][lane][16 * c]) = vn;
-            const uint32_t w[4] = {kn.x, kn.y, kn.z, kn.w};
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NB; ++c) *reinterpret_cast<uint4*>(&sV[warp][lane][16 * c]) = vn[c];
+#pragma unroll
+        for (int c = 0; c < 2 * NB; ++c) {
+            if (c >= C) break;
+            const uint32_t w[4] = {kn[c].x, kn[c].y, kn[c].z, kn[c].w};
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -433,9 +444,9 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
         for (int r = 0; r < R; ++r) {
             s[r] = in ? fmaf(s[r], ks.x, ks.y * sum_q[r]) : -INFINITY;
             const float to = fmaxf(m[r], warp_max(s[r])), use = to == -INFINITY ? 0.f : to;
-            scale_o[r] = m[r] == -INFINITY ? 0.f : expf(m[r] - use);
+            scale_o[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - use);
             m[r] = to;
-            p[r] = expf(s[r] - use);
+            p[r] = exp2f(s[r] - use);
             l[r] = fmaf(l[r], scale_o[r], p[r]);
             base[r] = fmaf(base[r], scale_o[r], p[r] * vs.y);
 #pragma unroll
@@ -474,29 +485,28 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
         if (lane == 0) { sM[warp][r] = m[r]; sL[warp][r] = l[r]; }
     }
     __syncthreads();
-    // a part without keys has nothing to weigh (its sums are 0); one whose keys all gave NaN has no maximum either, and stays NaN
-    auto weight = [](float mine, float all) { return mine == -INFINITY ? 1.f : expf(mine - all); };
+    // warp r joins the maxima and the weights' sums of row r: first the warps', then the blocks'
+    if (warp < R) {
+        const float mw = lane < W ? sM[lane][warp] : -INFINITY, all = warp_max(mw), f = lane < W ? part_weight(mw, all) : 0.f;
+        const float sum = warp_sum(lane < W ? f * sL[lane][warp] : 0.f);
+        if (lane < W) sF[warp][lane] = f;
+        if (lane == 0) { sAll[warp] = all; sSum[warp] = sum; }
+    }
+    __syncthreads();
     const size_t unit = (size_t)seq * gridDim.y + blockIdx.y, each = (size_t)R * (hd + 2);
     float* mine = partials + (unit * splits + split) * each;
-    for (int i = threadIdx.x; i < heads * hd; i += 32 * W) {
-        const int r = i / hd, d = i - r * hd;
-        float all = -INFINITY, sum = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) all = fmaxf(all, sM[w][r]);
+    for (int k = 0; k < R * DP / (32 * W); ++k) {
+        const int i = threadIdx.x + k * 32 * W, r = i / DP, d = i % DP;
+        if (r >= heads || d >= hd) continue;
+        float o = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = weight(sM[w][r], all);
-            sum = fmaf(f, sL[w][r], sum);
-            o = fmaf(f, sO[w][r][d], o);
-        }
-        if (used == 1) {
-            st_f(out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d, o / sum);
-        } else {
-            mine[i] = o;
-            if (d == 0) { mine[R * hd + r] = all; mine[R * hd + R + r] = sum; }
-        }
+        for (int w = 0; w < W; ++w) o = fmaf(sF[r][w], sO[w][r][d], o);
+        if (used == 1) st_f(out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d, o / sSum[r]);
+        else mine[r * hd + d] = o;
     }
     if (used == 1) return;
+    if (threadIdx.x < heads) { mine[R * hd + threadIdx.x] = sAll[threadIdx.x]; mine[R * hd + R + threadIdx.x] = sSum[threadIdx.x]; }
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -507,17 +517,37 @@ kv4_single_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ o
     if (!is_last) return;
     __threadfence();
     const float* parts = partials + unit * splits * each;
-    for (int i = threadIdx.x; i < heads * hd; i += 32 * W) {
-        const int r = i / hd, d = i - r * hd;
-        float all = -INFINITY, sum = 0.f, o = 0.f;
-        for (int c = 0; c < used; ++c) all = fmaxf(all, __ldcg(parts + c * each + R * hd + r));
-#pragma unroll 4
+    if (warp < heads) {
+        const float* ml = parts + R * hd + warp;
+        const bool in0 = lane < used, in1 = lane + 32 < used;
+        const float m0 = in0 ? __ldcg(ml + lane * each) : -INFINITY, m1 = in1 ? __ldcg(ml + (lane + 32) * each) : -INFINITY;
+        const float l0 = in0 ? __ldcg(ml + lane * each + R) : 0.f, l1 = in1 ? __ldcg(ml + (lane + 32) * each + R) : 0.f;
+        const float all = warp_max(fmaxf(m0, m1)), f0 = part_weight(m0, all), f1 = part_weight(m1, all);
+        const float sum = warp_sum(fmaf(f0, l0, f1 * l1));
+        sF[warp][lane] = f0;
+        sF[warp][lane + 32] = f1;
+        if (lane == 0) sSum[warp] = sum;
+    }
+    __syncthreads();
+    // four numbers a thread, the blocks' in their order
+    for (int i = threadIdx.x; i < heads * hd / 4; i += 32 * W) {
+        const int r = 4 * i / hd, d = 4 * i - r * hd;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
         for (int c = 0; c < used; ++c) {
-            const float f = weight(__ldcg(parts + c * each + R * hd + r), all);
-            sum = fmaf(f, __ldcg(parts + c * each + R * hd + R + r), sum);
-            o = fmaf(f, __ldcg(parts + c * each + i), o);
+            const float f = sF[r][c];
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(parts + c * each) + i);
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
         }
-        st_f(out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d, o / sum);
+        T* to = out + (size_t)seq * out_stride + (size_t)(head0 + r) * hd + d;
+        const float sum = sSum[r];
+        st_f(to, o.x / sum);
+        st_f(to + 1, o.y / sum);
+        st_f(to + 2, o.z / sum);
+        st_f(to + 3, o.w / sum);
     }
 }
 
@@ -820,7 +850,7 @@ VOB_EXPORT int vob_kv4_read(const void* cache, long long num_pages, const int* s
 
 // Attention in 32-bit arithmetic. Single tokens: `positions` int32 [S] (row s of q is request s); otherwise seq_starts int32 [S + 1] and
 // context_lens int32 [S]. `splits` blocks share a single token's keys, meeting in `partials` (S * G * ceil(H / G / 4) * splits * 4 * (hd + 2) floats; as
-// many as `partial_floats` lets there be) and `arrived` (S * G * ceil(H / G / 4) zeros).
+// many as `partial_floats` lets there be, 64 at most) and `arrived` (S * G * ceil(H / G / 4) zeros).
 VOB_EXPORT int vob_kv4_attend(const void* q, long long q_stride, void* out, long long out_stride, const void* cache, long long num_pages,
                               const int* block_tables, int max_pages, const int* positions, const int* seq_starts, const int* context_lens,
                               int S, int max_new, int H, int G, int hd, int page_size, float scale, int window, int code, int splits,
@@ -828,7 +858,7 @@ VOB_EXPORT int vob_kv4_attend(const void* q, long long q_stride, void* out, long
     if (S <= 0 || max_new <= 0) return 0;
     if (!sizes_ok(H, G, hd, page_size) || num_pages <= 0 || num_pages > 0x7fffffffLL || splits <= 0 || window < 0) return VOB_ERR_BAD_ARG;
     if (splits > 1) {
-        if (!partials || !arrived || !positions) return VOB_ERR_BAD_ARG;
+        if (!partials || !arrived || !positions || splits > MAX_SPLITS || ((uintptr_t)partials & 15)) return VOB_ERR_BAD_ARG;
         const long long units = (long long)S * G * ((H / G + SINGLE_ROWS - 1) / SINGLE_ROWS);
         if (counters < units) return VOB_ERR_BAD_ARG;
         splits = (int)max(1LL, min((long long)splits, partial_floats / (units * SINGLE_ROWS * (hd + 2))));
