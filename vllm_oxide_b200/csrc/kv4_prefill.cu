@@ -577,11 +577,13 @@ template <int HD> int launch(const Args& a, int S, long long row_tiles, cudaStre
     }
     // Blocks that share keys where there are few: as many as find room at once, one on an SM. (A cluster stays within a part of the GPU, and has fewer SMs to
     // choose from the larger it is: 74 of 2, 33 of 4 or 15 of 8 fit. 128 tokens behind 4,000 at 32/8 heads of 128, 16 blocks' worth of rows: 78.6 us unsplit,
-    // 39.6 by 4, 61.6 by 8; 16 tokens behind 8,000, 8 blocks' worth: 105, 40.1, 28.1.) Several requests count half of the longest's rows beyond one.
+    // 39.6 by 4, 61.6 by 8; 16 tokens behind 8,000, 8 blocks' worth: 105, 40.1, 28.1.) Requests beyond
+    // one count for a quarter, since lengths and contexts differ as a rule: 10 of 1 to 100 tokens behind up to 3,000 at 24/8 heads of 128 take 31.8 us, 45.5 where they
+    // count for a half; 4 of 100 behind 4,000 each, which are alike, 73 and 54.
     const long long sees = min((long long)a.max_pages * a.page_size, a.window ? (long long)a.window + 2 * BM : 0x7fffffffLL);
     int parts = 1;
     for (int i = 0; i < 3; ++i)
-        if (row_tiles * a.G * (S + 1) / 2 <= room[dev & 63][i] && (2 << i) * MIN_TILES * BN <= sees) parts = 2 << i;
+        if (row_tiles * a.G * (S + 3) / 4 <= room[dev & 63][i] && (2 << i) * MIN_TILES * BN <= sees) parts = 2 << i;
     const dim3 grid(a.G * parts, S, (unsigned)row_tiles);
     if (parts == 1) return vob_launch(kv4_prefill_kernel<HD, false>, grid, block, smem, stream, a);
     return launch_clusters(kv4_prefill_kernel<HD, true>, grid, parts, block, smem, stream, a);
