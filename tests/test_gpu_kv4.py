@@ -493,3 +493,73 @@ def test_two_streams_at_once(dtype):
     for per_stream in outs:
         for got in per_stream:
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_cache_beyond_32_bits_of_bytes(dtype):
+    """The same requests at both ends of a pool of 5 GB give the same bits."""
+    from vllm_oxide_b200 import kernels
+    H, G, hd, page, L, n = 8, 8, 128, 64, 500, 70
+    pages = 5 * 2 ** 30 // (G * page * plain.width(hd))
+    cache = torch.empty(pages, G, page, plain.width(hd), dtype=torch.uint8, device=DEV)
+    g = gen(31)
+    qkv = torch.randn(L, (H + 2 * G) * hd, generator=g).to(dtype).to(DEV)
+    positions = torch.arange(L, dtype=torch.int32, device=DEV)
+    need = -(-L // page)
+    got = []
+    for first in (0, pages - need):
+        table = torch.arange(first, first + need, dtype=torch.int32, device=DEV).view(1, -1)
+        slots = first * page + positions
+        q = torch.empty(L, H * hd, dtype=dtype, device=DEV)
+        kernels.kv4_append(qkv[:, :H * hd], qkv[:, H * hd:(H + G) * hd], qkv[:, (H + G) * hd:], positions, slots, freq(hd).to(DEV), cache, H, G, hd, q_out=q)
+        k, v = (torch.empty(L, G * hd, dtype=dtype, device=DEV) for _ in range(2))
+        kernels.kv4_read(cache, slots, k, v, G, hd)
+        one, many = torch.empty(1, H * hd, dtype=dtype, device=DEV), torch.empty(n, H * hd, dtype=dtype, device=DEV)
+        kernels.attn_decode_kv4(q[-1:], one, cache, table, positions[-1:], H, G, hd, hd ** -0.5, scratch=kernels.kv4_scratch(1, H, G, hd, DEV))
+        kernels.attn_prefill_kv4(q[-n:], many, cache, table, torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                                 torch.tensor([L - n], dtype=torch.int32, device=DEV), 1, n, H, G, hd, hd ** -0.5)
+        got.append((q, k, v, one, many))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and not a.isnan().any()
+    (q, k, v, one, many) = (x.cpu() for x in got[0])
+    ref, size, mag = plain.attend(q[-n:].view(n, H, hd), k.double().view(L, G, hd), v.double().view(L, G, hd), torch.arange(L - n, L), hd ** -0.5)
+    # (keys and values as read back are rounded to the type: half a step of them more)
+    tol = tolerance(ref, size, mag, None, dtype) + HALF[dtype] * (2 * size * (mag + ref.abs()) + mag)
+    assert ((many.double().view(n, H, hd) - ref).abs() <= tol).all() and ((one.double().view(1, H, hd) - ref[-1:]).abs() <= tol[-1:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_rows_at_odd_addresses_and_calls_without_rows(hd, dtype):
+    from vllm_oxide_b200 import kernels
+    H, G, page, lens, new = 8, 2, 16, [2000, 60], [9, 40]
+    cache, tables, keys, vals = paged(lens, G, hd, page, hd)
+    rows = sum(new)
+    wide = torch.randn(rows, H * hd + 3, generator=gen(41)).to(dtype).to(DEV)
+    q, out = wide[:, 1:1 + H * hd], torch.full((rows, H * hd + 5), 3.0, dtype=dtype, device=DEV)[:, 3:3 + H * hd]
+    starts = torch.tensor([0, new[0], rows], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([a - b for a, b in zip(lens, new)], dtype=torch.int32, device=DEV)
+    scratch = kernels.kv4_scratch(2, H, G, hd, DEV)
+
+    def portions(seqs, longest):
+        kernels.attn_prefill_kv4(q, out, cache, tables, starts, ctx, seqs, longest, H, G, hd, hd ** -0.5)
+
+    def single(n):
+        kernels.attn_decode_kv4(q[:n], out[:n], cache, tables, ctx, H, G, hd, hd ** -0.5, scratch=scratch)
+
+    portions(0, 40)
+    portions(2, 0)
+    single(0)
+    assert (out == 3).all()
+    portions(2, 40)
+    got, at = out.cpu().double(), 0
+    for s, n in enumerate(new):
+        ref, size, mag = plain.attend(q.cpu()[at:at + n].reshape(n, H, hd), keys[s], vals[s], torch.arange(lens[s] - n, lens[s]), hd ** -0.5)
+        assert ((got[at:at + n].view(n, H, hd) - ref).abs() <= tolerance(ref, size, mag, None, dtype)).all()
+        at += n
+    single(2)
+    got = out.cpu().double()
+    for s in range(2):
+        n = int(ctx[s]) + 1
+        ref, size, mag = plain.attend(q.cpu()[s:s + 1].reshape(1, H, hd), keys[s][:n], vals[s][:n], torch.tensor([n - 1]), hd ** -0.5)
+        assert ((got[s].view(1, H, hd) - ref).abs() <= tolerance(ref, size, mag, None, dtype)).all()
